@@ -18,7 +18,7 @@ own = False
 DEVICE = "cuda:0"
 PAGE = 64
 E4M3 = torch.float8_e4m3fn
-LOWEST, HIGHEST = -60, 120       # exponents of a vector's power of two
+LOWEST, HIGHEST = -60, 119       # exponents of a vector's power of two
 BIAS = 127
 
 
