@@ -58,6 +58,9 @@ LIBRARIES: Dict[str, tuple] = {
     "streams": ("streams.cu", []),
     "scaled_norm": ("scaled_norm.cu", []),
     "rglru": ("rglru.cu", []),
+    "kv_store": ("kv_store.cu", []),
+    "attention_tree": ("attention_tree.cu", []),
+    "logprobs": ("logprobs.cu", []),
 }
 
 _HEADERS = ["common.cuh", "page_map.cuh"]

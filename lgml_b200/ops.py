@@ -2923,3 +2923,252 @@ def paged_attention(q, batch, cache, out, n_heads: int, scale: float, window: in
             return prefill_attention(q, batch.positions, tiles, cache.block_table, cache.k, cache.v, out, n_heads, scale, window, status)
     return paged_attention_ref(q, batch.positions, batch.seq_of_token, cache.block_table, cache.k, cache.v, out, n_heads,
                                scale, window, status)
+
+
+# ----------------------------------------------------------------------------------------
+# a cache in eight bits, drafted tokens, log probabilities of given tokens
+# ----------------------------------------------------------------------------------------
+
+E4M3 = torch.float8_e4m3fn
+TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
+TREE_MAX_DIM = 128
+LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
+
+
+def _here(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor on the current device: the launch goes to that device's current stream."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise KernelError(f"{who}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _kv_pages(who: str, k_pages, v_pages, k_exps, v_exps) -> tuple:
+    """The checks of pages in bfloat16, or in e4m3 with an exponent a vector: their shape (pages, KV heads, page, head size)."""
+    eight = k_exps is not None or v_exps is not None
+    if eight and (k_exps is None or v_exps is None):
+        raise KernelError(f"{who}: exponents for the keys and the values, or for neither")
+    dt = E4M3 if eight else torch.bfloat16
+    _need(k_pages, "key pages", dt, 4)
+    _need(v_pages, "value pages", dt, 4)
+    if v_pages.shape != k_pages.shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise KernelError(f"{who}: key and value pages must be contiguous and of one shape ({tuple(k_pages.shape)}, {tuple(v_pages.shape)})")
+    for e in (k_exps, v_exps) if eight else ():
+        _need(e, "exponents", torch.uint8, 3)
+        if e.shape != k_pages.shape[:3] or not e.is_contiguous():
+            raise KernelError(f"{who}: exponents are contiguous [pages, KV heads, page], not {tuple(e.shape)}")
+    _here(who, k_pages, v_pages, k_exps, v_exps)
+    return tuple(k_pages.shape)
+
+
+def _status_word(who: str, status: torch.Tensor) -> None:
+    _need(status, "status", torch.int32)
+    if status.numel() != 1:
+        raise KernelError(f"{who}: the status is one int32")
+    _here(who, status)
+
+
+def _ints(who: str, what: str, t: torch.Tensor, n: Optional[int] = None) -> None:
+    _need(t, what, torch.int32, 1)
+    if not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise KernelError(f"{who}: {what} must be {'' if n is None else str(n) + ' '}contiguous int32 values (shape {tuple(t.shape)}, strides {t.stride()})")
+    _here(who, t)
+
+
+def _table(who: str, t: torch.Tensor) -> None:
+    _need(t, "block table", torch.int32, 2)
+    if not t.is_contiguous() or t.shape[1] < 1:
+        raise KernelError(f"{who}: the block table is contiguous with a column at least, not {tuple(t.shape)}")
+    _here(who, t)
+
+
+def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, block_table: torch.Tensor, inv_freq: torch.Tensor, n_rot: int, pairing: str,
+                  k_pages: torch.Tensor, v_pages: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, status: torch.Tensor,
+                  cells: Optional[torch.Tensor] = None, k_exps: Optional[torch.Tensor] = None, v_exps: Optional[torch.Tensor] = None, write_kv: bool = True,
+                  q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rope_kv_write`` with cells of their own and for pages of eight bits: rotates q and k by ``positions`` and stores k and v in ``cells``
+    (int32, the positions when None; drafted tokens that stand side by side share a position, not a cell).
+
+    ``k_exps`` / ``v_exps`` (uint8 [pages, KV heads, 64]) with pages in ``torch.float8_e4m3fn``: every key and value vector is stored as
+    codes and one power of two, e = clamp(ceil(log2(amax / 448)), -60, 119) over its finite entries, kept as e + 127; an entry is
+    rounded once, from float32, to half a step of four bits; NaN and infinities become NaN.  Without them the pages are bfloat16.
+    ``qkv``: bfloat16 [tokens, (H + 2 Hkv) D], or ``Partials``; q comes out in bfloat16, in ``q_out`` (never in place; made if None).
+    ``inv_freq``, ``n_rot``, ``pairing`` as for ``rope_kv_write``."""
+    who = "rope_kv_store"
+    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
+    width = (n_heads + 2 * n_kv_heads) * head_dim
+    bias = None
+    if isinstance(qkv, Partials):
+        src, bias = qkv.data, qkv.bias
+        _need(src, "qkv parts", torch.float32, 3)
+        if not src.is_contiguous() or src.shape[2] != width or src.shape[0] < 1:
+            raise KernelError(f"{who}: parts must be [parts, tokens, (H + 2 Hkv) D] and contiguous, not {tuple(src.shape)}")
+        n_parts, n, lds, stride = src.shape[0], src.shape[1], width, src.shape[1] * width
+        if bias is not None:
+            _need(bias, "qkv bias", torch.float32, 1)
+            if bias.numel() != width or not bias.is_contiguous():
+                raise KernelError(f"{who}: the bias has one value a column")
+    else:
+        src = qkv
+        _need(src, "qkv", torch.bfloat16, 2)
+        lds = _rows_contiguous(src, "qkv")
+        n_parts, n, stride = 1, src.shape[0], 0
+        if src.shape[1] != width:
+            raise KernelError(f"{who}: qkv is {tuple(src.shape)}, its width is not (H + 2 Hkv) D = {width}")
+    if (hkv, d) != (n_kv_heads, head_dim):
+        raise KernelError(f"{who}: pages {tuple(k_pages.shape)} do not fit {n_kv_heads} KV heads of {head_dim}")
+    if q_out is None:
+        q_out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=src.device)
+    _need(q_out, "rotated q", torch.bfloat16, 2)
+    ldq = _rows_contiguous(q_out, "rotated q")
+    if tuple(q_out.shape) != (n, n_heads * head_dim):
+        raise KernelError(f"{who}: rotated q is [tokens, H D], not {tuple(q_out.shape)}")
+    _ints(who, "positions", positions, n)
+    _ints(who, "request index of tokens", seq_of_token, n)
+    if cells is not None:
+        _ints(who, "cells", cells, n)
+    _table(who, block_table)
+    freq_lo = None
+    if inv_freq.dim() == 2:
+        if inv_freq.shape[0] != 2 or not inv_freq.is_contiguous():
+            raise KernelError(f"{who}: frequencies with low parts are a contiguous [2, n_rot / 2]")
+        inv_freq, freq_lo = inv_freq[0], inv_freq[1]
+    _need(inv_freq, "rotary frequencies", torch.float32, 1)
+    if pairing not in PAIRING:
+        raise KernelError(f"{who}: unknown pairing '{pairing}'")
+    if n_rot % 2 or n_rot < 0 or n_rot > head_dim or inv_freq.numel() < n_rot // 2 or not inv_freq.is_contiguous():
+        raise KernelError(f"{who}: n_rot {n_rot} must be even, at most head_dim, and have n_rot / 2 frequencies")
+    _status_word(who, status)
+    _here(who, src, bias, q_out, inv_freq)
+    fn = _fn("kv_store", "lgml_rope_kv_store", [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                                c_int, c_int, c_int, c_void_p, c_void_p])
+    _check("kv_store", fn(_ptr(src), dtype_code(src.dtype), lds, n_parts, stride, _ptr(bias), _ptr(q_out), ldq, _ptr(positions), _ptr(cells),
+                          _ptr(seq_of_token), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(inv_freq), _ptr(freq_lo), n_rot,
+                          PAIRING[pairing], _ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, n, n_heads, n_kv_heads, head_dim,
+                          1 if write_kv else 0, _ptr(status), _stream()), who)
+    return q_out
+
+
+def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, v_exps: torch.Tensor, pages: torch.Tensor, status: torch.Tensor,
+            k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
+    """Pages of eight bits back as bfloat16: page i of the results ([n, KV heads, 64, D], made if not given) is page ``pages[i]`` of the pool, every
+    code times its vector's power of two, which bfloat16 holds exactly.  A page number below zero leaves its page of the results as it
+    was; one past the pool too, and sets the status."""
+    who = "kv_read"
+    if k_exps is None or v_exps is None:
+        raise KernelError(f"{who}: pages in bfloat16 need no reading back (no exponents were given)")
+    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
+    _ints(who, "page list", pages)
+    shape = (pages.numel(), hkv, page, d)
+    outs = []
+    for out in (k_out, v_out):
+        if out is None:
+            out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
+        _need(out, "pages read back", torch.bfloat16, 4)
+        if tuple(out.shape) != shape or not out.is_contiguous():
+            raise KernelError(f"{who}: results are contiguous {shape}, not {tuple(out.shape)}")
+        outs.append(out)
+    _status_word(who, status)
+    _here(who, *outs)
+    fn = _fn("kv_store", "lgml_kv_read", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
+    _check("kv_store", fn(_ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, _ptr(pages), pages.numel(), _ptr(outs[0]), _ptr(outs[1]),
+                          hkv, d, _ptr(status), _stream()), who)
+    return outs[0], outs[1]
+
+
+def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64) -> int:
+    """Into how many ranges of pages ``tree_attention`` cuts a request's cells."""
+    blocks = max(n_seqs * n_kv_heads * -(-rows // (8 if rows <= 8 else 32)), 1)
+    pages = max(1, -(-longest // page))
+    return max(1, min(-(-pages // 2), (4 * sm_count()) // blocks, 64))
+
+
+def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
+                   v_pages: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, window: int, status: torch.Tensor, max_new_tokens: int,
+                   max_kv_len: int, k_exps: Optional[torch.Tensor] = None, v_exps: Optional[torch.Tensor] = None, visible: Optional[torch.Tensor] = None,
+                   n_splits: Optional[int] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of up to 64 new tokens a request over its cells, in bfloat16 pages or (with exponents) e4m3 ones.
+
+    Request s brings rows ``seq_start[s]`` to ``seq_start[s + 1]`` of q; cells 0 to ``seq_pos0[s]`` - 1 are old, cell ``seq_pos0[s]`` + j is its j-th
+    new token's.  ``visible`` (int64 [tokens], or None): bit j of a token's mask lets it see the request's j-th new token (its own bit
+    included, if it is to see itself); None: a chain, every token sees those up to itself.  Old cells are all seen; with ``window`` > 0 only
+    cells whose position is above the token's position - window (an old cell's position is its number).  A row that sees nothing is zeros.
+    Requests that bring more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
+    included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read."""
+    who = "tree_attention"
+    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
+    _need(q, "queries", torch.bfloat16, 2)
+    _need(out, "attention output", torch.bfloat16, 2)
+    ldq, ldo = _rows_contiguous(q, "queries"), _rows_contiguous(out, "attention output")
+    n = q.shape[0]
+    if n_heads < 1 or n_heads % hkv:
+        raise KernelError(f"{who}: {n_heads} heads are no multiple of {hkv} KV heads")
+    if q.shape[1] != n_heads * d or tuple(out.shape) != (n, n_heads * d):
+        raise KernelError(f"{who}: q {tuple(q.shape)} / out {tuple(out.shape)} do not fit {n_heads} heads of {d}")
+    if not 1 <= max_new_tokens <= TREE_TOKENS:
+        raise KernelError(f"{who}: {max_new_tokens} new tokens a request (1 to {TREE_TOKENS})")
+    _ints(who, "positions", positions, n)
+    _table(who, block_table)
+    S = block_table.shape[0]
+    _ints(who, "first rows of requests", seq_start, S + 1)
+    _ints(who, "old cells of requests", seq_pos0, S)
+    if visible is not None:
+        _need(visible, "masks", torch.int64, 1)
+        if visible.numel() != n or not visible.is_contiguous():
+            raise KernelError(f"{who}: one mask a token")
+    _status_word(who, status)
+    _here(who, q, out, visible, scratch)
+    if n_splits is None:
+        n_splits = tree_splits(S, hkv, max_new_tokens * (n_heads // hkv), max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page))
+    if n_splits > 1:
+        need = n * n_heads * n_splits * (d + 2)
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        _need(scratch, "scratch", torch.float32, 1)
+        if scratch.numel() < need or not scratch.is_contiguous():
+            raise KernelError(f"{who}: scratch of {scratch.numel()} floats, {need} needed")
+    fn = _fn("attention_tree", "lgml_tree_attention", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                                       c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                                                       c_void_p, c_void_p])
+    _check("attention_tree", fn(_ptr(q), ldq, _ptr(positions), _ptr(seq_start), _ptr(seq_pos0), _ptr(visible), _ptr(block_table), S, block_table.shape[1],
+                                _ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, _ptr(out), ldo, _ptr(scratch if n_splits > 1 else None),
+                                n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0), _ptr(status), _stream()), who)
+    return out
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs ranks entropies top_ids top_logprobs")
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: torch.Tensor) -> TokenLogprobs:
+    """Of every row of logits: the log probability of its given id, that id's rank (0: the best; among equals the lower id comes first), the entropy of
+    the row's distribution (natural units), and the ``top`` best ids with their log probabilities, ordered by (logit descending, id ascending).
+    Natural logarithms, float32; ids and ranks int32.  An id of -1 is none: its log probability is NaN, its rank -1; any other id outside the
+    vocabulary gives the same and sets the status.  A row with a NaN, an infinity of positive sign or nothing but negative ones has NaN figures."""
+    who = "token_logprobs"
+    _need(logits, "logits", torch.float32, 2)
+    n, v = logits.shape
+    if n and (logits.stride(1) != 1 or (n > 1 and logits.stride(0) < v)):
+        raise KernelError(f"{who}: logits must have dense rows (strides {logits.stride()})")
+    _ints(who, "ids", ids, n)
+    if not 0 <= top <= min(v, LOGPROBS_TOP) or v < 1:
+        raise KernelError(f"{who}: {top} alternatives (0 to min(vocabulary {v}, {LOGPROBS_TOP}))")
+    _status_word(who, status)
+    _here(who, logits)
+    dev = logits.device
+    out = TokenLogprobs(torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.float32, device=dev),
+                        torch.empty((n, top), dtype=torch.int32, device=dev), torch.empty((n, top), dtype=torch.float32, device=dev))
+    slices = _logprob_slices(n, v)
+    scratch = torch.empty(n * slices * (4 + 2 * top), dtype=torch.float32, device=dev) if slices > 1 else None
+    fn = _fn("logprobs", "lgml_token_logprobs", [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                 c_void_p, c_void_p])
+    _check("logprobs", fn(_ptr(logits), max(logits.stride(0), v), n, v, _ptr(ids), int(top), slices, _ptr(scratch), _ptr(out.logprobs), _ptr(out.ranks),
+                          _ptr(out.entropies), _ptr(out.top_ids), _ptr(out.top_logprobs), _ptr(status), _stream()), who)
+    return out
+
+
+@functools.lru_cache(maxsize=None)
+def _logprob_slices(n: int, v: int) -> int:
+    fn = csrc.load("logprobs").lgml_token_logprobs_slices
+    fn.argtypes, fn.restype = [c_int, c_int, c_int], c_int
+    return fn(n, v, sm_count())
