@@ -6,13 +6,14 @@
 // and the k largest x_i with their log p, ordered by (x descending, i ascending).  Taking u about the maximum, not about
 // zero, keeps the entropy exact when the logits are far from zero.
 //
-// A block has a slice of a row, in chunks of 8,192 logits that its threads hold in registers: every thread keeps m, s, u and
+// A block has a slice of a row, in chunks of 4,096 logits that its threads hold in registers: every thread keeps m, s, u and
 // its count (online: s and u are rescaled when m grows), joined once at the end.  The best k come from the same registers: of a
-// chunk only entries above the k-th best so far can be among them, and once some chunks are through those are few.  Where they are
-// many (the first chunk; rising logits) the k-th largest of the threads' own maxima is a bound that at least k entries reach
-// and, since entries are told apart by their index, that no more than k threads' 32 can: at most 32 k, which fit the buffer
-// whatever the order.  Entries are 64-bit keys (the float's order, then the lower index first), so the order of arrival in the
-// buffer changes nothing.  A row in several slices is joined by a second kernel, slice after slice.  All sums are float32.
+// chunk only entries above the k-th best so far can be among them, and once some chunks are through those are few.  Of the first chunk, a bound
+// that k entries reach: every warp's q-th largest of its threads' maxima, q = ceil(k / 8), and of the eight warps' the least.  Where that leaves
+// too many (equal logits; rising ones, later), the k-th largest of all the threads' maxima does not: entries are told apart by their index, so no
+// more than k threads reach it, with 16 entries each.  Entries are 64-bit keys (the float's order, then the lower index first), so the
+// order of arrival in the buffer changes nothing.
+// The slices of a row are a cluster, whose first block joins them, slice after slice, out of the others' shared memory.  All sums are float32.
 #include <math.h>
 
 #include "common.cuh"
@@ -21,21 +22,27 @@ LGML_DEFINE_LAST_ERROR(lgml_logprobs)
 
 namespace {
 constexpr int THREADS = 256;
-constexpr int PER = 32;                       // logits a thread holds
+constexpr int WARPS = THREADS / 32;
+constexpr int PER = 16;                       // logits a thread holds
 constexpr int CHUNK = THREADS * PER;
 constexpr int TOP_MAX = 32;
-constexpr int BUFFER = TOP_MAX * PER + TOP_MAX;      // candidates of a chunk, and the best so far
-constexpr int MAX_SLICES = 64;
+constexpr int BUFFER = TOP_MAX * PER;         // candidates of a chunk
+constexpr int MAX_SLICES = 16;                // blocks of a cluster
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long Key;
 
-// Larger keys come first: the float's order (NaN below everything, -0 as 0), then the lower index.  0: no entry.
-__device__ __forceinline__ Key key_of(float x, int i) {
-    const unsigned u = __float_as_uint(x + 0.f);
-    const unsigned o = x != x ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return ((Key)o << 32) | (unsigned)(0x7fffffff - i);
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
+// Larger keys come first: the float's order (NaN below everything, -0 as 0), then the lower index.  0: no entry.
+__device__ __forceinline__ unsigned order_of(float x) {
+    const unsigned u = __float_as_uint(x + 0.f);
+    return x != x ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ Key key_of(float x, int i) { return ((Key)order_of(x) << 32) | (unsigned)(0x7fffffff - i); }
 __device__ __forceinline__ int index_of(Key k) { return 0x7fffffff - (int)(unsigned)(k & 0xffffffffu); }
 __device__ __forceinline__ float value_of(Key k) {
     const unsigned o = (unsigned)(k >> 32);
@@ -49,7 +56,7 @@ struct Stats {
 __device__ __forceinline__ Stats about(Stats a, float M) {
     if (a.m == M || a.m == -INFINITY) return Stats{M, a.s, a.u};       // (nothing but -inf so far: s and u are 0, or NaN)
     const float d = fmaxf(a.m - M, -1e30f);        // (a maximum of the type's lowest value would make the product infinite, and infinity x 0 a NaN)
-    const float f = exp2f(d * LOG2E);
+    const float f = ex2(d * LOG2E);
     return Stats{M, a.s * f, (a.u + d * a.s) * f};
 }
 __device__ __forceinline__ Stats join(Stats a, Stats b) {
@@ -84,25 +91,71 @@ __device__ __forceinline__ void rank_keys(const Key *list, int n, Key *best, int
     for (int i = n + threadIdx.x; i < k; i += THREADS) best[i] = 0;
 }
 
-__global__ void __launch_bounds__(THREADS) logprobs_kernel(const float *__restrict__ logits, long long ld, int V, const int *__restrict__ ids, int top,
-                                                           int n_slices, int chunks_per_slice, int vec, float4 *__restrict__ part, Key *__restrict__ part_keys,
-                                                           Outputs out, int *__restrict__ status) {
+__device__ __forceinline__ unsigned block_of_cluster() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory"); }
+// The address, in the cluster, of what block `rank` has where this block has p.
+__device__ __forceinline__ uint32_t in_block(const void *p, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 load_there(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ Key load_key_there(uint32_t at) {
+    Key v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at));
+    return v;
+}
+
+struct Shared {
+    Key list[TOP_MAX + BUFFER];          // the best so far, then candidates; at the end, the slices' best
+    Key best[TOP_MAX];
+    Key thread_best[THREADS];
+    float4 mine;                         // of the slice: m, s, u, the count
+    Stats warp_stats[WARPS];
+    int warp_count[WARPS];
+    unsigned warp_bound[WARPS];
+    int n_list;
+    Key bound;
+};
+
+// Entries of the chunk that pass(x, i) go behind the best so far, as many as there is room for; returns how many there are.
+template <typename Pass>
+__device__ __forceinline__ int collect(Shared &sh, const float (&x)[PER], int first, int V, int top, Pass pass) {
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
+    if (threadIdx.x < top) sh.list[threadIdx.x] = sh.best[threadIdx.x];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = first + (j >> 2) * THREADS * 4 + (j & 3);
+        if (i < V && pass(x[j], i)) {
+            const int at = atomicAdd(&sh.n_list, 1);
+            if (at < BUFFER) sh.list[top + at] = key_of(x[j], i);
+        }
+    }
+    __syncthreads();
+    return sh.n_list;
+}
+
+__global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(const float *__restrict__ logits, long long ld, int V, const int *__restrict__ ids, int top,
+                                                              int n_slices, int chunks_per_slice, int vec, Outputs out, int *__restrict__ status) {
     pdl_trigger();
-    pdl_wait();
-    __shared__ Key list[BUFFER];
-    __shared__ Key best[TOP_MAX];
-    __shared__ Key thread_best[THREADS];
-    __shared__ Stats warp_stats[THREADS / 32];
-    __shared__ int warp_count[THREADS / 32];
-    __shared__ int n_list;
-    __shared__ Key bound;
-    const int r = blockIdx.x / n_slices, slice = blockIdx.x - r * n_slices, tid = threadIdx.x;
+    __shared__ __align__(16) Shared sh;
+    const int r = blockIdx.x / n_slices, slice = n_slices > 1 ? (int)block_of_cluster() : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float *row = logits + (size_t)r * ld;
+    pdl_wait();
     const int id = act_load(ids + r);
     const bool known = id >= 0 && id < V;
     if (!known && id != -1 && tid == 0) atomicExch(status, 1);
     const float x_id = known ? act_load(row + id) : __int_as_float(0x7fffffff);
-    if (tid < TOP_MAX) best[tid] = 0;
+    if (tid < TOP_MAX) sh.best[tid] = 0;
     __syncthreads();
 
     Stats st{-INFINITY, 0.f, 0.f};
@@ -110,81 +163,82 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const float *__restri
     for (int c = 0; c < chunks_per_slice; ++c) {
         const int base = (slice * chunks_per_slice + c) * CHUNK;
         if (base >= V) break;
+        const int first = base + tid * 4;            // a thread's j-th entry is first + (j / 4) * 4 * THREADS + j % 4
         float x[PER];
-        const bool whole = vec && V - base >= CHUNK;
+        if (vec && V - base >= CHUNK) {
 #pragma unroll
-        for (int j = 0; j < PER / 4; ++j) {
-            const int at = base + (j * THREADS + tid) * 4;
-            if (whole) {
-                const float4 v = act_load(reinterpret_cast<const float4 *>(row + at));
+            for (int j = 0; j < PER / 4; ++j) {
+                const float4 v = act_load(reinterpret_cast<const float4 *>(row + first + j * THREADS * 4));
                 x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
-            } else {
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * j + e] = at + e < V ? act_load(row + at + e) : -INFINITY;
+            for (int j = 0; j < PER; ++j) {
+                const int i = first + (j >> 2) * THREADS * 4 + (j & 3);
+                x[j] = i < V ? act_load(row + i) : -INFINITY;
             }
         }
         // ---- sums ----
-        float M = st.m;
+        float largest = x[0];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) M = fmaxf(M, x[j]);
-        st = about(st, M);
-        const float ref = M == -INFINITY ? 0.f : M;
+        for (int j = 1; j < PER; ++j) largest = fmaxf(largest, x[j]);
+        if (largest > st.m) st = about(st, largest);
+        const float ref = st.m == -INFINITY ? 0.f : st.m;
+        int above = 0, from = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const float d = x[j] - ref, w = exp2f(d * LOG2E);
+            const float d = x[j] - ref, w = ex2(d * LOG2E);
             st.s += w;
             st.u += fmaxf(d, -1e30f) * w;
-            const int i = base + ((j >> 2) * THREADS + tid) * 4 + (j & 3);
-            greater += x[j] > x_id || (x[j] == x_id && i < id);
+            above += x[j] > x_id, from += x[j] >= x_id;
         }
+        if (from != above)              // (equal ones: the id itself, and a few)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) above += x[j] == x_id && first + (j >> 2) * THREADS * 4 + (j & 3) < id;
+        greater += above;
         if (top == 0) continue;
         // ---- the best ----
         // (entries of later chunks have larger indices: an equal value does not displace the k-th best)
-        const Key kth = best[top - 1];
-        int mine = 0;
+        const Key kth = sh.best[top - 1];
+        const unsigned kth_order = (unsigned)(kth >> 32);          // 0: not k yet, or NaNs among them
+        int n;
+        if (kth_order != 0) {
+            const float least = value_of(kth);
+            if (!__syncthreads_or(largest > least)) continue;
+            n = collect(sh, x, first, V, top, [=](float v, int) { return v > least; });
+        } else {
+            unsigned left = 0, q_th = 0;              // (places past the vocabulary are none)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = base + ((j >> 2) * THREADS + tid) * 4 + (j & 3);
-            mine += i < V && key_of(x[j], i) > kth;
+            for (int j = 0; j < PER; ++j)
+                if (first + (j >> 2) * THREADS * 4 + (j & 3) < V) left = max(left, order_of(x[j]));
+            for (int q = 0; q < (top + WARPS - 1) / WARPS; ++q) {
+                q_th = __reduce_max_sync(0xffffffffu, left);
+                if (lane == __ffs(__ballot_sync(0xffffffffu, left == q_th)) - 1) left = 0;
+            }
+            if (lane == 0) sh.warp_bound[warp] = q_th;
+            __syncthreads();
+            unsigned bound = sh.warp_bound[0];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) bound = min(bound, sh.warp_bound[w]);
+            n = collect(sh, x, first, V, top, [=](float v, int i) { return order_of(v) >= bound && key_of(v, i) > kth; });
         }
-        int total = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if ((tid & 31) == 0) warp_count[tid >> 5] = total;
-        if (!__syncthreads_or(mine)) continue;
-        total = 0;
-        for (int w = 0; w < THREADS / 32; ++w) total += warp_count[w];
-        Key floor_key = kth;            // entries above it go to the buffer
-        if (total > TOP_MAX * PER) {
+        if (n > BUFFER) {
             Key local = 0;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int i = base + ((j >> 2) * THREADS + tid) * 4 + (j & 3);
+                const int i = first + (j >> 2) * THREADS * 4 + (j & 3);
                 if (i < V) local = max(local, key_of(x[j], i));
             }
-            thread_best[tid] = local;
+            sh.thread_best[tid] = local;
             __syncthreads();
             int before = 0;
-            for (int j = 0; j < THREADS; ++j) before += thread_best[j] > local || (thread_best[j] == local && j < tid);
-            if (before == top - 1) bound = local;
+            for (int j = 0; j < THREADS; ++j) before += sh.thread_best[j] > local || (sh.thread_best[j] == local && j < tid);
+            if (before == top - 1) sh.bound = local;
             __syncthreads();
-            if (bound != 0 && bound - 1 > floor_key) floor_key = bound - 1;       // entries from the bound on
+            const Key bound = sh.bound;
+            n = collect(sh, x, first, V, top, [=](float v, int i) { const Key k = key_of(v, i); return k > kth && k >= bound; });
         }
-        if (tid == 0) n_list = 0;
-        __syncthreads();
-        if (tid < top) list[tid] = best[tid];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = base + ((j >> 2) * THREADS + tid) * 4 + (j & 3);
-            const Key k = key_of(x[j], i);
-            if (i < V && k > floor_key) {
-                const int at = atomicAdd(&n_list, 1);
-                if (at < TOP_MAX * PER) list[top + at] = k;
-            }
-        }
-        __syncthreads();
-        const int n = top + min(n_list, TOP_MAX * PER);
-        rank_keys(list, n, best, top);
+        rank_keys(sh.list, top + min(n, BUFFER), sh.best, top);
         __syncthreads();
     }
 
@@ -194,96 +248,66 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const float *__restri
         st = join(st, Stats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.u, o)});
         greater += __shfl_xor_sync(0xffffffffu, greater, o);
     }
-    __syncthreads();
-    if ((tid & 31) == 0) warp_stats[tid >> 5] = st, warp_count[tid >> 5] = greater;
+    if (lane == 0) sh.warp_stats[warp] = st, sh.warp_count[warp] = greater;
     __syncthreads();
     if (tid == 0) {
-        st = warp_stats[0], greater = warp_count[0];
-        for (int w = 1; w < THREADS / 32; ++w) st = join(st, warp_stats[w]), greater += warp_count[w];
-        warp_stats[0] = st;
-        if (n_slices == 1) write_row(out, r, id, known, x_id, st, greater);
-        else part[(size_t)r * n_slices + slice] = make_float4(st.m, st.s, st.u, __int_as_float(greater));
+        for (int w = 1; w < WARPS; ++w) st = join(st, sh.warp_stats[w]), greater += sh.warp_count[w];
+        sh.mine = make_float4(st.m, st.s, st.u, __int_as_float(greater));
     }
-    __syncthreads();
-    if (tid >= top) return;
-    if (n_slices == 1) {
-        const Key k = best[tid];
-        out.top_ids[(size_t)r * top + tid] = index_of(k);
-        out.top_logprobs[(size_t)r * top + tid] = value_of(k) - warp_stats[0].m - logf(warp_stats[0].s);
+    // ---- and the slices ----
+    if (n_slices > 1) {
+        cluster_sync();
+        if (slice == 0) {
+            for (int i = tid; i < n_slices * top; i += THREADS) sh.list[i] = load_key_there(in_block(sh.best + i % top, i / top));
+            __syncthreads();
+            rank_keys(sh.list, n_slices * top, sh.thread_best, top);
+            if (tid == 0) {
+                for (int i = 1; i < n_slices; ++i) {
+                    const float4 v = load_there(in_block(&sh.mine, i));
+                    st = join(st, Stats{v.x, v.y, v.z});
+                    greater += __float_as_int(v.w);
+                }
+                sh.mine = make_float4(st.m, st.s, st.u, 0.f);
+            }
+        }
+        cluster_sync();                 // (the others' shared memory is read until here)
+        if (slice != 0) return;
     } else {
-        part_keys[((size_t)r * n_slices + slice) * top + tid] = best[tid];
+        __syncthreads();
     }
-}
-
-// A row's slices together, in their order.
-__global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const float *__restrict__ logits, long long ld, int V, const int *__restrict__ ids, int top,
-                                                                int n_slices, const float4 *__restrict__ part, const Key *__restrict__ part_keys,
-                                                                Outputs out) {
-    pdl_trigger();
-    pdl_wait();
-    __shared__ Key list[MAX_SLICES * TOP_MAX];
-    __shared__ Key best[TOP_MAX];
-    __shared__ Stats slices[MAX_SLICES];
-    __shared__ int counts[MAX_SLICES];
-    const int r = blockIdx.x, tid = threadIdx.x;
-    for (int i = tid; i < n_slices; i += THREADS) {
-        const float4 p = act_load(part + (size_t)r * n_slices + i);
-        slices[i] = Stats{p.x, p.y, p.z};
-        counts[i] = __float_as_int(p.w);
-    }
-    const int n = n_slices * top;
-    for (int i = tid; i < n; i += THREADS) list[i] = __ldcg(part_keys + (size_t)r * n + i);
-    __syncthreads();
-    rank_keys(list, n, best, top);
-    if (tid == 0) {
-        Stats st = slices[0];
-        int greater = counts[0];
-        for (int i = 1; i < n_slices; ++i) st = join(st, slices[i]), greater += counts[i];
-        const int id = act_load(ids + r);
-        const bool known = id >= 0 && id < V;
-        write_row(out, r, id, known, known ? act_load(logits + (size_t)r * ld + id) : 0.f, st, greater);
-        slices[0] = st;
-    }
-    __syncthreads();
+    if (tid == 0) write_row(out, r, id, known, x_id, st, greater);
     if (tid < top) {
-        const Key k = best[tid];
+        const Key k = n_slices > 1 ? sh.thread_best[tid] : sh.best[tid];
         out.top_ids[(size_t)r * top + tid] = index_of(k);
-        out.top_logprobs[(size_t)r * top + tid] = value_of(k) - slices[0].m - logf(slices[0].s);
+        out.top_logprobs[(size_t)r * top + tid] = value_of(k) - sh.mine.x - logf(sh.mine.y);
     }
 }
 }  // namespace
 
-// Into how many slices a row is cut, and the bytes of scratch that takes.
+// Into how many slices (a power of two) a row is cut.
 LGML_API int lgml_token_logprobs_slices(int n_rows, int V, int n_sms) {
     const int chunks = (V + CHUNK - 1) / CHUNK;
-    int slices = n_rows > 0 ? (4 * n_sms) / n_rows : 1;
-    if (slices > chunks) slices = chunks;
-    if (slices > MAX_SLICES) slices = MAX_SLICES;
-    if (slices < 1) slices = 1;
-    const int per = (chunks + slices - 1) / slices;
-    return (chunks + per - 1) / per;
-}
-LGML_API long long lgml_token_logprobs_scratch(int n_rows, int top, int n_slices) {
-    return n_slices <= 1 ? 0 : (long long)n_rows * n_slices * (16 + 8 * top);
+    int slices = 1;
+    while (slices < MAX_SLICES && 2 * slices <= chunks && (long long)n_rows * 2 * slices <= 4 * n_sms) slices *= 2;
+    return slices;
 }
 
-LGML_API int lgml_token_logprobs(const float *logits, long long ld, int n_rows, int V, const int *ids, int top, int n_slices, void *scratch, float *logprob,
-                                 int *rank, float *entropy, int *top_ids, float *top_logprobs, int *status, cudaStream_t stream) {
+LGML_API int lgml_token_logprobs(const float *logits, long long ld, int n_rows, int V, const int *ids, int top, int n_slices, float *logprob, int *rank,
+                                 float *entropy, int *top_ids, float *top_logprobs, int *status, cudaStream_t stream) {
     LGML_REQUIRE(n_rows >= 0 && V > 0 && ld >= V, "token_logprobs: %d rows of %d logits, %lld apart", n_rows, V, ld);
     LGML_REQUIRE(V <= 1 << 30, "token_logprobs: a vocabulary of %d", V);
     LGML_REQUIRE(top >= 0 && top <= TOP_MAX && top <= V, "token_logprobs: %d alternatives (0 to %d, at most the vocabulary)", top, TOP_MAX);
-    LGML_REQUIRE(n_slices >= 1 && n_slices <= MAX_SLICES, "token_logprobs: %d slices (1 to %d)", n_slices, MAX_SLICES);
-    LGML_REQUIRE(n_slices == 1 || (scratch != nullptr && ((uintptr_t)scratch & 15) == 0), "token_logprobs: several slices need scratch memory on 16 bytes");
+    LGML_REQUIRE(n_slices >= 1 && n_slices <= MAX_SLICES && (n_slices & (n_slices - 1)) == 0, "token_logprobs: %d slices (a power of two up to %d)", n_slices,
+                 MAX_SLICES);
     LGML_REQUIRE((long long)n_rows * n_slices <= 0x7fffffffLL, "token_logprobs: too many rows");
     if (n_rows == 0) return 0;
     const int chunks = (V + CHUNK - 1) / CHUNK, per = (chunks + n_slices - 1) / n_slices;
     const int vec = ld % 4 == 0 && ((uintptr_t)logits & 15) == 0;
-    float4 *part = (float4 *)scratch;
-    Key *keys = (Key *)(part + (size_t)n_rows * n_slices);
     const Outputs out{logprob, rank, entropy, top_ids, top_logprobs};
-    lgml_launch(logprobs_kernel, dim3(n_rows * n_slices), THREADS, 0, stream, logits, ld, V, ids, top, n_slices, per, vec, part, keys, out, status);
-    int rc = lgml_launch_status("token_logprobs");
-    if (rc || n_slices == 1) return rc;
-    lgml_launch(logprobs_join_kernel, dim3(n_rows), THREADS, 0, stream, logits, ld, V, ids, top, n_slices, part, keys, out);
-    return lgml_launch_status("token_logprobs_join");
+    if (n_slices > 8) {
+        cudaError_t e = cudaFuncSetAttribute(logprobs_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) LGML_FAIL("token_logprobs: no clusters of %d: %s", n_slices, cudaGetErrorString(e));
+    }
+    lgml_launch_cluster(logprobs_kernel, dim3(n_rows * n_slices), THREADS, 0, stream, n_slices, logits, ld, V, ids, top, n_slices, per, vec, out, status);
+    return lgml_launch_status("token_logprobs");
 }

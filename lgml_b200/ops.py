@@ -2935,51 +2935,57 @@ TREE_MAX_DIM = 128
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
 
 
-def _here(who: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor on the current device: the launch goes to that device's current stream."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+def _are(who: str, dev: int, dtype: torch.dtype, ndim: int, names: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All of them (None: not given) contiguous tensors of this type and number of dimensions on device ``dev``.  (A call checks a dozen tensors;
+    where all is well that is four questions each.)"""
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
-            raise KernelError(f"{who}: a tensor is on {t.device}, the current device is cuda:{dev}")
+        if t is not None and (t.dtype is not dtype or t.dim() != ndim or t.get_device() != dev or not t.is_contiguous()):
+            which = [name for name, x in zip(names.split(", "), tensors) if x is t][0]
+            _need(t, f"{who}: {which}", dtype, ndim)
+            if t.get_device() != dev:
+                raise KernelError(f"{who}: {which} are on {t.device}, not on cuda:{dev}")
+            raise KernelError(f"{who}: {which} must be contiguous (shape {tuple(t.shape)}, strides {t.stride()})")
 
 
-def _kv_pages(who: str, k_pages, v_pages, k_exps, v_exps) -> tuple:
+def _current(who: str, dev: int) -> None:
+    """Launches go to the current device's current stream: the tensors' device has to be that one."""
+    if dev != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise KernelError(f"{who}: the tensors are on cuda:{dev}, which is not the current device")
+
+
+def _device_of(who: str, t: torch.Tensor, what: str) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        _need(t, f"{who}: {what}")
+    _current(who, dev)
+    return dev
+
+
+def _kv_pages(who: str, dev: int, k_pages, v_pages, k_exps, v_exps) -> tuple:
     """The checks of pages in bfloat16, or in e4m3 with an exponent a vector: their shape (pages, KV heads, page, head size)."""
-    eight = k_exps is not None or v_exps is not None
-    if eight and (k_exps is None or v_exps is None):
+    if (k_exps is None) != (v_exps is None):
         raise KernelError(f"{who}: exponents for the keys and the values, or for neither")
-    dt = E4M3 if eight else torch.bfloat16
-    _need(k_pages, "key pages", dt, 4)
-    _need(v_pages, "value pages", dt, 4)
-    if v_pages.shape != k_pages.shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
-        raise KernelError(f"{who}: key and value pages must be contiguous and of one shape ({tuple(k_pages.shape)}, {tuple(v_pages.shape)})")
-    for e in (k_exps, v_exps) if eight else ():
-        _need(e, "exponents", torch.uint8, 3)
-        if e.shape != k_pages.shape[:3] or not e.is_contiguous():
-            raise KernelError(f"{who}: exponents are contiguous [pages, KV heads, page], not {tuple(e.shape)}")
-    _here(who, k_pages, v_pages, k_exps, v_exps)
-    return tuple(k_pages.shape)
+    _are(who, dev, torch.bfloat16 if k_exps is None else E4M3, 4, "key pages, value pages", k_pages, v_pages)
+    shape = k_pages.shape
+    if v_pages.shape != shape:
+        raise KernelError(f"{who}: key and value pages must be of one shape ({tuple(shape)}, {tuple(v_pages.shape)})")
+    if k_exps is not None:
+        _are(who, dev, torch.uint8, 3, "key exponents, value exponents", k_exps, v_exps)
+        if k_exps.shape != shape[:3] or v_exps.shape != shape[:3]:
+            raise KernelError(f"{who}: exponents are [pages, KV heads, page], not {tuple(k_exps.shape)} and {tuple(v_exps.shape)}")
+    return shape
 
 
-def _status_word(who: str, status: torch.Tensor) -> None:
-    _need(status, "status", torch.int32)
-    if status.numel() != 1:
-        raise KernelError(f"{who}: the status is one int32")
-    _here(who, status)
-
-
-def _ints(who: str, what: str, t: torch.Tensor, n: Optional[int] = None) -> None:
-    _need(t, what, torch.int32, 1)
-    if not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise KernelError(f"{who}: {what} must be {'' if n is None else str(n) + ' '}contiguous int32 values (shape {tuple(t.shape)}, strides {t.stride()})")
-    _here(who, t)
-
-
-def _table(who: str, t: torch.Tensor) -> None:
-    _need(t, "block table", torch.int32, 2)
-    if not t.is_contiguous() or t.shape[1] < 1:
-        raise KernelError(f"{who}: the block table is contiguous with a column at least, not {tuple(t.shape)}")
-    _here(who, t)
+def _rows_on(who: str, dev: int, t: torch.Tensor, what: str, dtype: torch.dtype, width: int, n: Optional[int] = None) -> int:
+    """Row stride of a tensor [n, width] with dense rows on device ``dev``."""
+    shape = t.shape
+    if t.dtype is not dtype or t.get_device() != dev or len(shape) != 2 or shape[1] != width or (n is not None and shape[0] != n):
+        _need(t, f"{who}: {what}", dtype, 2)
+        raise KernelError(f"{who}: {what} must be [{'tokens' if n is None else n}, {width}] on cuda:{dev}, not {tuple(shape)} on {t.device}")
+    stride = t.stride()
+    if stride[1] != 1 or stride[0] < width:
+        raise KernelError(f"{who}: {what} must have dense rows (shape {tuple(shape)}, strides {stride})")
+    return stride[0]
 
 
 def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, block_table: torch.Tensor, inv_freq: torch.Tensor, n_rot: int, pairing: str,
@@ -2995,58 +3001,55 @@ def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, bloc
     ``qkv``: bfloat16 [tokens, (H + 2 Hkv) D], or ``Partials``; q comes out in bfloat16, in ``q_out`` (never in place; made if None).
     ``inv_freq``, ``n_rot``, ``pairing`` as for ``rope_kv_write``."""
     who = "rope_kv_store"
-    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
+    dev = _device_of(who, k_pages, "key pages")
+    n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)
+    if hkv != n_kv_heads or d != head_dim:
+        raise KernelError(f"{who}: pages {tuple(k_pages.shape)} do not fit {n_kv_heads} KV heads of {head_dim}")
     width = (n_heads + 2 * n_kv_heads) * head_dim
-    bias = None
     if isinstance(qkv, Partials):
-        src, bias = qkv.data, qkv.bias
-        _need(src, "qkv parts", torch.float32, 3)
-        if not src.is_contiguous() or src.shape[2] != width or src.shape[0] < 1:
-            raise KernelError(f"{who}: parts must be [parts, tokens, (H + 2 Hkv) D] and contiguous, not {tuple(src.shape)}")
-        n_parts, n, lds, stride = src.shape[0], src.shape[1], width, src.shape[1] * width
+        src, bias, src_type = qkv.data, qkv.bias, F32
+        _are(who, dev, torch.float32, 3, "qkv parts", src)
+        n_parts, n, lds = src.shape
+        stride = n * lds
+        if lds != width or n_parts < 1:
+            raise KernelError(f"{who}: parts must be [parts, tokens, (H + 2 Hkv) D], not {tuple(src.shape)}")
         if bias is not None:
-            _need(bias, "qkv bias", torch.float32, 1)
-            if bias.numel() != width or not bias.is_contiguous():
+            _are(who, dev, torch.float32, 1, "qkv bias", bias)
+            if bias.numel() != width:
                 raise KernelError(f"{who}: the bias has one value a column")
     else:
-        src = qkv
-        _need(src, "qkv", torch.bfloat16, 2)
-        lds = _rows_contiguous(src, "qkv")
-        n_parts, n, stride = 1, src.shape[0], 0
-        if src.shape[1] != width:
-            raise KernelError(f"{who}: qkv is {tuple(src.shape)}, its width is not (H + 2 Hkv) D = {width}")
-    if (hkv, d) != (n_kv_heads, head_dim):
-        raise KernelError(f"{who}: pages {tuple(k_pages.shape)} do not fit {n_kv_heads} KV heads of {head_dim}")
+        src, bias, src_type, n_parts, stride = qkv, None, BF16, 1, 0
+        lds = _rows_on(who, dev, src, "qkv", torch.bfloat16, width)
+        n = src.shape[0]
     if q_out is None:
         q_out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=src.device)
-    _need(q_out, "rotated q", torch.bfloat16, 2)
-    ldq = _rows_contiguous(q_out, "rotated q")
-    if tuple(q_out.shape) != (n, n_heads * head_dim):
-        raise KernelError(f"{who}: rotated q is [tokens, H D], not {tuple(q_out.shape)}")
-    _ints(who, "positions", positions, n)
-    _ints(who, "request index of tokens", seq_of_token, n)
-    if cells is not None:
-        _ints(who, "cells", cells, n)
-    _table(who, block_table)
-    freq_lo = None
+    ldq = _rows_on(who, dev, q_out, "rotated q", torch.bfloat16, n_heads * head_dim, n)
+    _are(who, dev, torch.int32, 1, "positions, request index of tokens, cells, status", positions, seq_of_token, cells, status)
+    _are(who, dev, torch.int32, 2, "block table", block_table)
+    if positions.numel() != n or seq_of_token.numel() != n or (cells is not None and cells.numel() != n) or status.numel() != 1:
+        raise KernelError(f"{who}: one position, request index and cell for each of {n} tokens, and one status")
+    low = 0
     if inv_freq.dim() == 2:
-        if inv_freq.shape[0] != 2 or not inv_freq.is_contiguous():
-            raise KernelError(f"{who}: frequencies with low parts are a contiguous [2, n_rot / 2]")
-        inv_freq, freq_lo = inv_freq[0], inv_freq[1]
-    _need(inv_freq, "rotary frequencies", torch.float32, 1)
+        _are(who, dev, torch.float32, 2, "rotary frequencies", inv_freq)
+        if inv_freq.shape[0] != 2:
+            raise KernelError(f"{who}: frequencies with low parts are [2, n_rot / 2]")
+        n_freq = inv_freq.shape[1]
+        low = inv_freq.data_ptr() + 4 * n_freq
+    else:
+        _are(who, dev, torch.float32, 1, "rotary frequencies", inv_freq)
+        n_freq = inv_freq.numel()
     if pairing not in PAIRING:
         raise KernelError(f"{who}: unknown pairing '{pairing}'")
-    if n_rot % 2 or n_rot < 0 or n_rot > head_dim or inv_freq.numel() < n_rot // 2 or not inv_freq.is_contiguous():
+    if n_rot % 2 or n_rot < 0 or n_rot > head_dim or n_freq < n_rot // 2:
         raise KernelError(f"{who}: n_rot {n_rot} must be even, at most head_dim, and have n_rot / 2 frequencies")
-    _status_word(who, status)
-    _here(who, src, bias, q_out, inv_freq)
+    seqs, blocks = block_table.shape
     fn = _fn("kv_store", "lgml_rope_kv_store", [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                                 c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                                 c_int, c_int, c_int, c_void_p, c_void_p])
-    _check("kv_store", fn(_ptr(src), dtype_code(src.dtype), lds, n_parts, stride, _ptr(bias), _ptr(q_out), ldq, _ptr(positions), _ptr(cells),
-                          _ptr(seq_of_token), _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(inv_freq), _ptr(freq_lo), n_rot,
-                          PAIRING[pairing], _ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, n, n_heads, n_kv_heads, head_dim,
-                          1 if write_kv else 0, _ptr(status), _stream()), who)
+    _check("kv_store", fn(src.data_ptr(), src_type, lds, n_parts, stride, _ptr(bias), q_out.data_ptr(), ldq, positions.data_ptr(), _ptr(cells),
+                          seq_of_token.data_ptr(), block_table.data_ptr(), seqs, blocks, inv_freq.data_ptr(), low, n_rot, PAIRING[pairing],
+                          k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, n, n_heads, n_kv_heads, head_dim,
+                          1 if write_kv else 0, status.data_ptr(), _stream()), who)
     return q_out
 
 
@@ -3058,23 +3061,22 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     who = "kv_read"
     if k_exps is None or v_exps is None:
         raise KernelError(f"{who}: pages in bfloat16 need no reading back (no exponents were given)")
-    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
-    _ints(who, "page list", pages)
-    shape = (pages.numel(), hkv, page, d)
-    outs = []
-    for out in (k_out, v_out):
-        if out is None:
-            out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
-        _need(out, "pages read back", torch.bfloat16, 4)
-        if tuple(out.shape) != shape or not out.is_contiguous():
-            raise KernelError(f"{who}: results are contiguous {shape}, not {tuple(out.shape)}")
-        outs.append(out)
-    _status_word(who, status)
-    _here(who, *outs)
+    dev = _device_of(who, k_pages, "key pages")
+    n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)
+    _are(who, dev, torch.int32, 1, "page list, status", pages, status)
+    n = pages.numel()
+    shape = (n, hkv, page, d)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
+    _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
+    if k_out.shape != shape or v_out.shape != shape or status.numel() != 1:
+        raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}, and the status is one int32")
     fn = _fn("kv_store", "lgml_kv_read", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
-    _check("kv_store", fn(_ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, _ptr(pages), pages.numel(), _ptr(outs[0]), _ptr(outs[1]),
-                          hkv, d, _ptr(status), _stream()), who)
-    return outs[0], outs[1]
+    _check("kv_store", fn(k_pages.data_ptr(), v_pages.data_ptr(), k_exps.data_ptr(), v_exps.data_ptr(), n_pages, page, pages.data_ptr(), n, k_out.data_ptr(),
+                          v_out.data_ptr(), hkv, d, status.data_ptr(), _stream()), who)
+    return k_out, v_out
 
 
 def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64) -> int:
@@ -3097,43 +3099,40 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     Requests that bring more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
     included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read."""
     who = "tree_attention"
-    n_pages, hkv, page, d = _kv_pages(who, k_pages, v_pages, k_exps, v_exps)
-    _need(q, "queries", torch.bfloat16, 2)
-    _need(out, "attention output", torch.bfloat16, 2)
-    ldq, ldo = _rows_contiguous(q, "queries"), _rows_contiguous(out, "attention output")
-    n = q.shape[0]
+    dev = _device_of(who, k_pages, "key pages")
+    n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)
     if n_heads < 1 or n_heads % hkv:
         raise KernelError(f"{who}: {n_heads} heads are no multiple of {hkv} KV heads")
-    if q.shape[1] != n_heads * d or tuple(out.shape) != (n, n_heads * d):
-        raise KernelError(f"{who}: q {tuple(q.shape)} / out {tuple(out.shape)} do not fit {n_heads} heads of {d}")
+    ldq = _rows_on(who, dev, q, "queries", torch.bfloat16, n_heads * d)
+    n = q.shape[0]
+    ldo = _rows_on(who, dev, out, "attention output", torch.bfloat16, n_heads * d, n)
     if not 1 <= max_new_tokens <= TREE_TOKENS:
         raise KernelError(f"{who}: {max_new_tokens} new tokens a request (1 to {TREE_TOKENS})")
-    _ints(who, "positions", positions, n)
-    _table(who, block_table)
-    S = block_table.shape[0]
-    _ints(who, "first rows of requests", seq_start, S + 1)
-    _ints(who, "old cells of requests", seq_pos0, S)
+    _are(who, dev, torch.int32, 2, "block table", block_table)
+    seqs, blocks = block_table.shape
+    _are(who, dev, torch.int32, 1, "positions, first rows of requests, old cells of requests, status", positions, seq_start, seq_pos0, status)
+    if positions.numel() != n or seq_start.numel() != seqs + 1 or seq_pos0.numel() != seqs or status.numel() != 1:
+        raise KernelError(f"{who}: one position for each of {n} tokens, {seqs + 1} first rows and {seqs} counts of old cells for {seqs} requests, and one status")
     if visible is not None:
-        _need(visible, "masks", torch.int64, 1)
-        if visible.numel() != n or not visible.is_contiguous():
+        _are(who, dev, torch.int64, 1, "masks", visible)
+        if visible.numel() != n:
             raise KernelError(f"{who}: one mask a token")
-    _status_word(who, status)
-    _here(who, q, out, visible, scratch)
     if n_splits is None:
-        n_splits = tree_splits(S, hkv, max_new_tokens * (n_heads // hkv), max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page))
+        n_splits = tree_splits(seqs, hkv, max_new_tokens * (n_heads // hkv), max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page))
     if n_splits > 1:
         need = n * n_heads * n_splits * (d + 2)
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-        _need(scratch, "scratch", torch.float32, 1)
-        if scratch.numel() < need or not scratch.is_contiguous():
+        _are(who, dev, torch.float32, 1, "scratch", scratch)
+        if scratch.numel() < need:
             raise KernelError(f"{who}: scratch of {scratch.numel()} floats, {need} needed")
     fn = _fn("attention_tree", "lgml_tree_attention", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                                        c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                                                        c_void_p, c_void_p])
-    _check("attention_tree", fn(_ptr(q), ldq, _ptr(positions), _ptr(seq_start), _ptr(seq_pos0), _ptr(visible), _ptr(block_table), S, block_table.shape[1],
-                                _ptr(k_pages), _ptr(v_pages), _ptr(k_exps), _ptr(v_exps), n_pages, page, _ptr(out), ldo, _ptr(scratch if n_splits > 1 else None),
-                                n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0), _ptr(status), _stream()), who)
+    _check("attention_tree", fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
+                                blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
+                                scratch.data_ptr() if n_splits > 1 else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
+                                status.data_ptr(), _stream()), who)
     return out
 
 
@@ -3146,25 +3145,25 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: to
     Natural logarithms, float32; ids and ranks int32.  An id of -1 is none: its log probability is NaN, its rank -1; any other id outside the
     vocabulary gives the same and sets the status.  A row with a NaN, an infinity of positive sign or nothing but negative ones has NaN figures."""
     who = "token_logprobs"
+    dev = _device_of(who, logits, "logits")
     _need(logits, "logits", torch.float32, 2)
     n, v = logits.shape
-    if n and (logits.stride(1) != 1 or (n > 1 and logits.stride(0) < v)):
+    ld, one = logits.stride()
+    if n and (one != 1 or (n > 1 and ld < v)):
         raise KernelError(f"{who}: logits must have dense rows (strides {logits.stride()})")
-    _ints(who, "ids", ids, n)
+    _are(who, dev, torch.int32, 1, "ids, status", ids, status)
+    if ids.numel() != n or status.numel() != 1:
+        raise KernelError(f"{who}: one id for each of {n} rows, and one status")
     if not 0 <= top <= min(v, LOGPROBS_TOP) or v < 1:
         raise KernelError(f"{who}: {top} alternatives (0 to min(vocabulary {v}, {LOGPROBS_TOP}))")
-    _status_word(who, status)
-    _here(who, logits)
-    dev = logits.device
-    out = TokenLogprobs(torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.float32, device=dev),
-                        torch.empty((n, top), dtype=torch.int32, device=dev), torch.empty((n, top), dtype=torch.float32, device=dev))
-    slices = _logprob_slices(n, v)
-    scratch = torch.empty(n * slices * (4 + 2 * top), dtype=torch.float32, device=dev) if slices > 1 else None
+    # all results in one allocation, each kind in one run: log p, rank, entropy, then ids and log p of the best
+    flat = torch.empty(n * (3 + 2 * top), dtype=torch.float32, device=logits.device)
+    at, ints = flat.data_ptr(), flat.view(torch.int32)
     fn = _fn("logprobs", "lgml_token_logprobs", [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                 c_void_p, c_void_p])
-    _check("logprobs", fn(_ptr(logits), max(logits.stride(0), v), n, v, _ptr(ids), int(top), slices, _ptr(scratch), _ptr(out.logprobs), _ptr(out.ranks),
-                          _ptr(out.entropies), _ptr(out.top_ids), _ptr(out.top_logprobs), _ptr(status), _stream()), who)
-    return out
+                                                 c_void_p])
+    _check("logprobs", fn(logits.data_ptr(), max(ld, v), n, v, ids.data_ptr(), int(top), _logprob_slices(n, v), at, at + 4 * n, at + 8 * n, at + 12 * n,
+                          at + 12 * n + 4 * n * top, status.data_ptr(), _stream()), who)
+    return TokenLogprobs(flat[:n], ints[n:2 * n], flat[2 * n:3 * n], ints[3 * n:3 * n + n * top].view(n, top), flat[3 * n + n * top:3 * n + 2 * n * top].view(n, top))
 
 
 @functools.lru_cache(maxsize=None)
