@@ -10,9 +10,11 @@
 // Rows: a request's (token, head of the KV head) pairs, 8 NT of them a block.  The keys are the M side of the tensor-core tiles
 // (mma.sync m16n8k16), so that a token's few heads fill an N of 8:
 //     S^T[16 keys, 8 rows] = K[16, D] . Q^T        O^T[D, 8 rows] += V^T[D, 16] . P^T
-// A warp takes 16 cells at a time and holds their part of everything in registers; keys and values go from memory to the fragments
-// without shared memory, since the order of the D entries inside a product, and of the D rows of O^T, is free: a thread's entries of
-// a row are neighbours, so its loads are 16 bytes wide, and a warp's loads whole rows.
+// Each of a block's four warps is a pipeline of its own: of every page it takes a quarter, 16 cells, through a ring of stages in shared memory that
+// 16-byte asynchronous copies fill (rows 16 bytes apart from a multiple of 128, so that neither products' reads meet a bank twice).  The order of the D entries
+// inside a product, and of the D rows of O^T, is free: a thread's entries of a row are neighbours, and it reads 16 bytes at a time.
+// The ranges of a request's pages are a cluster of up to 8 blocks, which join through one another's shared memory; where there are more,
+// through scratch memory and a second kernel.
 //
 // e4m3: codes are exact in float16, so the products are of float16 (q is scaled per row by a power of two so that its largest
 // entry is in [2^14, 2^15): rounding it to float16 loses nothing above 2^-39 of that).  A key's power of two multiplies its score, exactly.  A value's joins
@@ -34,7 +36,7 @@ constexpr int PAGE = 64;
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int MAX_NEW = 64;             // bits of a mask
-constexpr int MAX_SPLITS = 256;
+constexpr int MAX_SPLITS = 256, MAX_CLUSTER = 8;
 
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 __device__ __forceinline__ unsigned half2_of_codes(unsigned short two) {
@@ -57,20 +59,47 @@ __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, uns
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N 32-bit words from p, by loads of W words (what has been written by the kernels ahead goes through L2).
-template <int N, int W>
-__device__ __forceinline__ void load_words(unsigned (&r)[N], const uint8_t *p, bool there) {
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy_16(uint32_t dst, const void *src, bool there) {
+    const int bytes = there ? 16 : 0;            // 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ unsigned block_of_cluster() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory"); }
+// What block `rank` of the cluster has where this block has p.
+__device__ __forceinline__ float2 load_there(const float *p, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
+}
+
+// N 32-bit words of shared memory, at most four at a time.
+template <int N>
+__device__ __forceinline__ void read_words(unsigned (&r)[N], const uint8_t *p) {
+    if (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += W) {
-        if (W == 4) {
-            const uint4 v = there ? __ldcg(reinterpret_cast<const uint4 *>(p + 4 * i)) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < N; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + 4 * i);
             r[i] = v.x, r[(i + 1) % N] = v.y, r[(i + 2) % N] = v.z, r[(i + 3) % N] = v.w;
-        } else if (W == 2) {
-            const uint2 v = there ? __ldcg(reinterpret_cast<const uint2 *>(p + 4 * i)) : make_uint2(0, 0);
-            r[i] = v.x, r[(i + 1) % N] = v.y;
-        } else {
-            r[i] = there ? __ldcg(reinterpret_cast<const unsigned *>(p + 4 * i)) : 0u;
         }
+    } else if (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r[0] = v.x, r[N - 1] = v.y;
+    } else {
+        r[0] = *reinterpret_cast<const unsigned *>(p);
     }
 }
 
@@ -79,30 +108,42 @@ __device__ __forceinline__ void load_words(unsigned (&r)[N], const uint8_t *p, b
 //   values: thread g = lane / 4 has, of every 8 E neighbouring entries, E: as rows g and g + 8 of E / 2 products
 template <int KS, bool Q8> struct Cut {
     static constexpr int SIZE = Q8 ? 1 : 2;
-    static constexpr int KE = Q8 ? (KS % 4 == 0 ? 16 : KS % 2 == 0 ? 8 : 4) : (KS % 2 == 0 ? 8 : 4);
+    static constexpr int KE = Q8 ? (KS % 8 == 0 ? 32 : KS % 4 == 0 ? 16 : KS % 2 == 0 ? 8 : 4) : (KS % 4 == 0 ? 16 : KS % 2 == 0 ? 8 : 4);
     static constexpr int VE = Q8 ? (KS % 8 == 0 ? 16 : KS % 4 == 0 ? 8 : KS % 2 == 0 ? 4 : 2) : (KS % 4 == 0 ? 8 : KS % 2 == 0 ? 4 : 2);
-    static constexpr int KW = KE * SIZE / 4, VW = VE * SIZE / 4;       // words of a load (a value's 2 codes of e4m3: half a word)
+    static constexpr int KW = KE * SIZE / 4, VW = VE * SIZE / 4;       // words of these (a value's 2 codes of e4m3: half a word)
+    static constexpr int ROW = KS * 16 * SIZE, PITCH = ROW + 16;       // bytes of a row, and from row to row in a stage
+    static constexpr int STAGE = 32 * PITCH + 32;                      // 16 keys, 16 values, their exponents
+    static constexpr int STAGES = 3;
     static __device__ __forceinline__ int key_entry(int ks, int c) { return (ks / (KE / 4)) * 4 * KE + c * KE + (ks % (KE / 4)) * 4; }
     static __device__ __forceinline__ int value_entry(int mt, int g) { return (mt / (VE / 2)) * 8 * VE + g * VE + (mt % (VE / 2)) * 2; }
 };
+
+// What a part with maximum m counts for beside others up to M (nothing seen: 0, or NaN, which stays one).
+__device__ __forceinline__ float share_of(float m, float M) { return m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M); }
+__device__ __forceinline__ void store_row(__nv_bfloat16 *dst, float2 o, float l) {
+    const float inv = 1.f / l;
+    *reinterpret_cast<__nv_bfloat162 *>(dst) = l == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o.x * inv, o.y * inv);
+}
 
 template <int KS, int NT, bool Q8>
 __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     const __nv_bfloat16 *__restrict__ q, int ldq, const int *__restrict__ positions, const int *__restrict__ seq_start, const int *__restrict__ seq_pos0,
     const long long *__restrict__ visible, const int *__restrict__ block_table, int max_blocks, const uint8_t *__restrict__ k_pages,
     const uint8_t *__restrict__ v_pages, const uint8_t *__restrict__ k_exps, const uint8_t *__restrict__ v_exps, int n_pages, __nv_bfloat16 *__restrict__ out,
-    int ldo, float *__restrict__ part_o, float2 *__restrict__ part_ml, int n_splits, int n_tokens, int H, int Hkv, int n_chunks, int limit, float scale,
-    int window, int *__restrict__ status) {
+    int ldo, float *__restrict__ part_o, float2 *__restrict__ part_ml, int n_splits, int clustered, int n_tokens, int H, int Hkv, int n_chunks, int limit,
+    float scale, int window, int *__restrict__ status) {
     pdl_trigger();
     constexpr int D = KS * 16, ROWS = 8 * NT;
     using C = Cut<KS, Q8>;
-    extern __shared__ __align__(16) float merge[];                 // [WARPS][ROWS][D + 2] at the end
+    extern __shared__ __align__(16) uint8_t smem[];                // the warps' stages; at the end [WARPS][ROWS][D + 2] floats
     __shared__ int row_pos[ROWS];
     __shared__ long long row_mask[ROWS];
+    __shared__ __align__(8) float fin[ROWS][2];
+    __shared__ int stage_page[WARPS][C::STAGES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-    const int s = blockIdx.x, kvh = blockIdx.y / n_chunks, chunk = blockIdx.y - kvh * n_chunks, split = blockIdx.z;
-    pdl_wait();
-    const int row0 = act_load(seq_start + s), n = act_load(seq_start + s + 1) - row0, pos0 = act_load(seq_pos0 + s);
+    const int s = blockIdx.x / n_splits, split = blockIdx.x - s * n_splits, kvh = blockIdx.y / n_chunks, chunk = blockIdx.y - kvh * n_chunks;
+    // (the step's description, down to the first pages' numbers, is read while the kernels ahead may still run)
+    const int row0 = early_int(seq_start + s), n = early_int(seq_start + s + 1) - row0, pos0 = early_int(seq_pos0 + s);
     const int group = H / Hkv, n_rows = n * group, r0 = chunk * ROWS;
     if (n <= 0 || n > limit || r0 >= n_rows) return;
     if (row0 < 0 || row0 + n > n_tokens || pos0 < 0) {
@@ -111,12 +152,55 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     }
     if (tid < ROWS) {
         const int r = min(r0 + tid, n_rows - 1), tok = r / group;
-        row_pos[tid] = act_load(positions + row0 + tok);
+        row_pos[tid] = early_int(positions + row0 + tok);
         row_mask[tid] = visible ? __ldcg(visible + row0 + tok) : (long long)(~0ull >> (63 - tok));
     }
     __syncthreads();
 
+    // the cells of this split, in whole pages
+    const int n_cells = pos0 + n;
+    int low = 0, all_from = 0;              // none of the rows sees a cell below the first, every row sees the old cells from the second on
+    if (window > 0) {
+        int lowest = row_pos[0], highest = row_pos[0];
+        for (int i = 1; i < ROWS; ++i) lowest = min(lowest, row_pos[i]), highest = max(highest, row_pos[i]);
+        low = min(max(lowest - window + 1, 0), pos0);
+        all_from = highest - window + 1;
+    }
+    const int first_page = low / PAGE, end_page = (n_cells + PAGE - 1) / PAGE;
+    const int pps = (end_page - first_page + n_splits - 1) / n_splits;
+    const int pb = first_page + split * pps, n_it = max(min(pps, end_page - pb), 0);
+
+    // ---- the copies: this warp's quarter of page pb + it into stage it % STAGES ----
+    uint8_t *ring = smem + (size_t)warp * C::STAGES * C::STAGE;
+    auto table_from = [&](int it) { return it + lane < n_it && pb + it + lane < max_blocks ? early_int(block_table + (size_t)s * max_blocks + pb + it + lane) : -1; };
+    int pages_ahead = table_from(0);        // the table's entry for iteration (it / 32) * 32 + lane
+    auto fetch = [&](int it) {
+        if ((it & 31) == 0 && it > 0) pages_ahead = table_from(it);
+        int page = __shfl_sync(0xffffffffu, pages_ahead, it & 31);
+        const int cell0 = (pb + it) * PAGE + warp * 16, left = n_cells - cell0;
+        if (left <= 0 || cell0 + 16 <= low) {
+            page = -1;                      // nothing there that a row could see
+        } else if (page < 0 || page >= n_pages) {
+            if (lane == 0) atomicExch(status, 3);
+            page = -1;
+        }
+        uint8_t *stage = ring + (it % C::STAGES) * C::STAGE;
+        if (lane == 0) stage_page[warp][it % C::STAGES] = page;
+        if (page < 0) return;
+        const size_t vec0 = ((size_t)page * Hkv + kvh) * PAGE + warp * 16;
+        const uint8_t *kt = k_pages + vec0 * C::ROW, *vt = v_pages + vec0 * C::ROW;
+        constexpr int PER_ROW = C::ROW / 16;
+#pragma unroll
+        for (int u = lane; u < 16 * PER_ROW; u += 32) {
+            const int row = u / PER_ROW, col = (u - row * PER_ROW) * 16;
+            const uint32_t to = smem_u32(stage + row * C::PITCH + col);
+            copy_16(to, kt + row * C::ROW + col, row < left);
+            copy_16(to + 16 * C::PITCH, vt + row * C::ROW + col, row < left);
+        }
+        if (Q8 && lane < 2) copy_16(smem_u32(stage + 32 * C::PITCH + 16 * lane), (lane ? v_exps : k_exps) + vec0, true);
+    };
     // Q^T as B fragments: row g of n-tile nt, the entries that the keys' fragments have in this thread
+    pdl_wait();
     unsigned qb[NT][KS][2];
     float q_unscale[NT][2];          // 2^-(row's scaling) of rows 2 c and 2 c + 1
 #pragma unroll
@@ -124,20 +208,30 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
         const int r = r0 + nt * 8 + g;
         const bool there = r < n_rows;
         const __nv_bfloat16 *qrow = q + (size_t)(row0 + (there ? r / group : 0)) * ldq + (size_t)(kvh * group + (there ? r % group : 0)) * D;
-        float amax = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const unsigned *p = reinterpret_cast<const unsigned *>(qrow + C::key_entry(ks, c));
             qb[nt][ks][0] = there ? act_load(p) : 0u;
             qb[nt][ks][1] = there ? act_load(p + 1) : 0u;
-            if (Q8)
+        }
+    }
+#pragma unroll
+    for (int it = 0; it < C::STAGES - 1; ++it) {
+        if (it < n_it) fetch(it);
+        copies_commit();
+    }
+
+    if (Q8)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float amax = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&qb[nt][ks][e]));
                     amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
-        }
-        if (Q8) {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             // 2^x so that amax 2^x is in [2^14, 2^15); x within what float32 holds (an infinite amax: whatever, the row is NaN)
@@ -154,21 +248,6 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
             q_unscale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);            // thread (g = 2 c, any) has row 2 c
             q_unscale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
         }
-    }
-
-    // the cells of this split, in whole pages
-    const int n_cells = pos0 + n;
-    int low = 0, all_from = 0;              // none of the rows sees a cell below the first, every row sees the old cells from the second on
-    if (window > 0) {
-        int lowest = row_pos[0], highest = row_pos[0];
-        for (int i = 1; i < ROWS; ++i) lowest = min(lowest, row_pos[i]), highest = max(highest, row_pos[i]);
-        low = min(max(lowest - window + 1, 0), pos0);
-        all_from = highest - window + 1;
-    }
-    const int first_page = low / PAGE, end_page = (n_cells + PAGE - 1) / PAGE;
-    const int pps = (end_page - first_page + n_splits - 1) / n_splits;
-    const int pb = first_page + split * pps, pe = min(pb + pps, end_page);
-    const int t_end = min(4 * pe, (n_cells + 15) / 16);
 
     const float scale_log2 = scale * 1.4426950408889634f;
     float m_run[NT][2], l_run[NT][2], oacc[NT][KS][4];
@@ -179,65 +258,46 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
         for (int i = 0; i < KS; ++i) oacc[nt][i][0] = oacc[nt][i][1] = oacc[nt][i][2] = oacc[nt][i][3] = 0.f;
     }
 
-    for (int tile = 4 * pb + warp; tile < t_end; tile += WARPS) {
-        const int cell0 = tile * 16;
-        const int blk = tile >> 2;
-        int page = blk < max_blocks ? act_load(block_table + (size_t)s * max_blocks + blk) : -1;
-        if (page < 0 || page >= n_pages) {
-            if (lane == 0 && cell0 + 16 > low) atomicExch(status, 3);
+    for (int it = 0; it < n_it; ++it) {
+        if (it + C::STAGES - 1 < n_it) fetch(it + C::STAGES - 1);
+        copies_commit();
+        copies_wait<C::STAGES - 1>();
+        __syncwarp();
+        const int page = stage_page[warp][it % C::STAGES];
+        if (page < 0) {
+            __syncwarp();
             continue;
         }
-        const size_t vec0 = ((size_t)page * Hkv + kvh) * PAGE + (tile & 3) * 16;
-        const uint8_t *kt = k_pages + vec0 * D * C::SIZE, *vt = v_pages + vec0 * D * C::SIZE;
-        const int left = n_cells - cell0;                          // cells of the tile that there are
-        const int vkey[4] = {2 * c, 2 * c + 1, 2 * c + 8, 2 * c + 9};
-
-        // ---- loads: keys g and g + 8; values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 ----
-        constexpr int KL = KS * 4 / C::KE, VL = KS * 2 / C::VE;          // loads of a row
-        unsigned kw[2][KL][C::KW];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < KL; ++i)
-                load_words<C::KW, C::KW>(kw[h][i], kt + ((size_t)(g + 8 * h) * D + i * 4 * C::KE + c * C::KE) * C::SIZE, g + 8 * h < left);
-        constexpr int VWORDS = C::VW > 0 ? C::VW : 1;
-        unsigned vw[4][VL][VWORDS];
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const uint8_t *p = vt + ((size_t)vkey[h] * D + i * 8 * C::VE + g * C::VE) * C::SIZE;
-                if (C::VW > 0) load_words<VWORDS, VWORDS>(vw[h][i], p, vkey[h] < left);
-                else vw[h][i][0] = vkey[h] < left ? (unsigned)__ldcg(reinterpret_cast<const unsigned short *>(p)) : 0u;
-            }
+        const uint8_t *stage = ring + (it % C::STAGES) * C::STAGE, *vs = stage + 16 * C::PITCH, *es = stage + 32 * C::PITCH;
+        const int cell0 = (pb + it) * PAGE + warp * 16, left = n_cells - cell0;
         int ke[2] = {0, 0}, ve[2] = {0, 0};
         if (Q8)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (g + 8 * h < left) {
-                    ke[h] = min((int)__ldcg(k_exps + vec0 + g + 8 * h), 246) - 127;          // (246: the largest that is written)
-                    ve[h] = min((int)__ldcg(v_exps + vec0 + g + 8 * h), 246) - 127;
-                }
+            for (int h = 0; h < 2; ++h) {
+                ke[h] = min((int)es[g + 8 * h], 246) - 127;          // (246: the largest that is written)
+                ve[h] = min((int)es[16 + g + 8 * h], 246) - 127;
+            }
 
         // ---- S^T ----
-        float sc[NT][4];
+        // (in two sums where there is one tile of rows: a product waits for the one before it in its sum)
+        constexpr int SUMS = NT == 1 ? 2 : 1;
+        float sc[NT][4], sums[SUMS][NT][4] = {};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+        for (int i = 0; i < KS * 4 / C::KE; ++i) {
+            unsigned kw[2][C::KW];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int i = ks / (C::KE / 4), u = ks % (C::KE / 4);
-            unsigned a[4];
+            for (int h = 0; h < 2; ++h) read_words(kw[h], stage + (g + 8 * h) * C::PITCH + (i * 4 * C::KE + c * C::KE) * C::SIZE);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (Q8) {
-                    const unsigned w = kw[h][i][u];
-                    a[h] = half2_of_codes((unsigned short)w), a[2 + h] = half2_of_codes((unsigned short)(w >> 16));
-                } else {
-                    a[h] = kw[h][i][(2 * u) % C::KW], a[2 + h] = kw[h][i][(2 * u + 1) % C::KW];
+            for (int u = 0; u < C::KE / 4; ++u) {
+                unsigned a[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (Q8) a[h] = half2_of_codes((unsigned short)kw[h][u % C::KW]), a[2 + h] = half2_of_codes((unsigned short)(kw[h][u % C::KW] >> 16));
+                    else a[h] = kw[h][(2 * u) % C::KW], a[2 + h] = kw[h][(2 * u + 1) % C::KW];
                 }
-            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<Q8>(sc[nt], a[0], a[1], a[2], a[3], qb[nt][ks][0], qb[nt][ks][1]);
+                for (int nt = 0; nt < NT; ++nt) mma<Q8>(sums[u % SUMS][nt], a[0], a[1], a[2], a[3], qb[nt][i * (C::KE / 4) + u][0], qb[nt][i * (C::KE / 4) + u][1]);
+            }
         }
         // ---- which of them are seen: bit i of seen[nt] for sc[nt][i] ----
         const bool whole = cell0 + 16 <= pos0 && cell0 >= all_from;
@@ -268,7 +328,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = sc[nt][i] * kf[i >> 1];
+                float x = (SUMS == 2 ? sums[0][nt][i] + sums[SUMS - 1][nt][i] : sums[0][nt][i]) * kf[i >> 1];
                 if (Q8) x = x * q_unscale[nt][i & 1] + (float)ve[i >> 1];
                 sc[nt][i] = (seen[nt] >> i) & 1 ? x : -INFINITY;
                 mx[i & 1] = fmaxf(mx[i & 1], sc[nt][i]);
@@ -279,7 +339,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
                 mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
                 mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
                 const float m_new = fmaxf(m_run[nt][e], mx[e]);
-                corr[nt][e] = m_new == m_run[nt][e] ? 1.f : exp2f(m_run[nt][e] - m_new);
+                corr[nt][e] = m_new == m_run[nt][e] ? 1.f : ex2(m_run[nt][e] - m_new);
                 grown |= m_new != m_run[nt][e];
                 m_run[nt][e] = m_new;
                 l_run[nt][e] *= corr[nt][e];
@@ -287,7 +347,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float m = m_run[nt][i & 1];
-                pr[nt][i] = exp2f(sc[nt][i] - (m == -INFINITY ? 0.f : m));        // (unseen: exp2(-inf) = 0)
+                pr[nt][i] = ex2(sc[nt][i] - (m == -INFINITY ? 0.f : m));          // (unseen: exp2(-inf) = 0)
             }
             unsigned lo, hi;
             if (Q8) {
@@ -317,16 +377,11 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
         // ---- values that are not finite, among cells that not every row sees ----
         if (!whole) {
             bool odd = false;
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int i = 0; i < VL; ++i)
-#pragma unroll
-                    for (int w = 0; w < VWORDS; ++w) {
-                        const unsigned x = vw[h][i][w];
-                        if (Q8) odd |= (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
-                        else odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-                    }
+            for (int u = lane; u < 16 * C::ROW / 4; u += 32) {
+                const unsigned x = *reinterpret_cast<const unsigned *>(vs + (u / (C::ROW / 4)) * C::PITCH + (u % (C::ROW / 4)) * 4);
+                if (Q8) odd |= (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+                else odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+            }
             if (__any_sync(0xffffffffu, odd)) {
                 for (int key = 0; key < min(left, 16); ++key) {
 #pragma unroll
@@ -340,10 +395,10 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
                             const int d = C::value_entry(mt, g);
                             float2 v;
                             if (Q8) {
-                                const unsigned h2 = half2_of_codes(__ldcg(reinterpret_cast<const unsigned short *>(vt + (size_t)key * D + d)));
+                                const unsigned h2 = half2_of_codes(*reinterpret_cast<const unsigned short *>(vs + key * C::PITCH + d));
                                 v = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
                             } else {
-                                const unsigned b2 = __ldcg(reinterpret_cast<const unsigned *>(vt + ((size_t)key * D + d) * 2));
+                                const unsigned b2 = *reinterpret_cast<const unsigned *>(vs + key * C::PITCH + 2 * d);
                                 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&b2));
                             }
                             if (bits & 1u) oacc[nt][mt][0] += p_a * v.x, oacc[nt][mt][2] += p_a * v.y;
@@ -351,32 +406,45 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
                         }
                     }
                 }
+                __syncwarp();
                 continue;
             }
         }
         // ---- O^T += V^T P^T ----
+        constexpr int VWORDS = C::VW > 0 ? C::VW : 1;
 #pragma unroll
-        for (int mt = 0; mt < KS; ++mt) {
-            const int i = mt / (C::VE / 2), u = mt % (C::VE / 2);
-            unsigned a[4];
+        for (int i = 0; i < KS * 2 / C::VE; ++i) {
+            unsigned vw[4][VWORDS];               // of cells 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {             // keys 2 c and 2 c + 1, then 2 c + 8 and 2 c + 9
-                if (Q8) {
-                    const unsigned wa = vw[2 * h][i][u / 2], wb = vw[2 * h + 1][i][u / 2];
-                    const unsigned both = __byte_perm(wa, wb, u % 2 ? 0x7362 : 0x5140);          // entry of one key, of the other, the next entry's
-                    a[2 * h] = half2_of_codes((unsigned short)both), a[2 * h + 1] = half2_of_codes((unsigned short)(both >> 16));
-                } else {
-                    const unsigned wa = vw[2 * h][i][u], wb = vw[2 * h + 1][i][u];
-                    a[2 * h] = __byte_perm(wa, wb, 0x5410), a[2 * h + 1] = __byte_perm(wa, wb, 0x7632);
-                }
+            for (int h = 0; h < 4; ++h) {
+                const uint8_t *p = vs + (2 * c + (h & 1) + (h >> 1) * 8) * C::PITCH + (i * 8 * C::VE + g * C::VE) * C::SIZE;
+                if (C::VW > 0) read_words(vw[h], p);
+                else vw[h][0] = *reinterpret_cast<const unsigned short *>(p);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<Q8>(oacc[nt][mt], a[0], a[1], a[2], a[3], pb0[nt], pb1[nt]);
+            for (int u = 0; u < C::VE / 2; ++u) {
+                unsigned a[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (Q8) {
+                        const unsigned both = __byte_perm(vw[2 * h][u / 2], vw[2 * h + 1][u / 2], u % 2 ? 0x7362 : 0x5140);      // an entry of both cells, the next entry's
+                        a[2 * h] = half2_of_codes((unsigned short)both), a[2 * h + 1] = half2_of_codes((unsigned short)(both >> 16));
+                    } else {
+                        a[2 * h] = __byte_perm(vw[2 * h][u % VWORDS], vw[2 * h + 1][u % VWORDS], 0x5410);
+                        a[2 * h + 1] = __byte_perm(vw[2 * h][u % VWORDS], vw[2 * h + 1][u % VWORDS], 0x7632);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma<Q8>(oacc[nt][i * (C::VE / 2) + u], a[0], a[1], a[2], a[3], pb0[nt], pb1[nt]);
+            }
         }
+        __syncwarp();
     }
+    copies_wait<0>();
+    __syncthreads();                        // every warp is done with its stages
 
     // ---- the four warps together ----
-    float *mine = merge + (size_t)warp * ROWS * (D + 2);
+    float *merge = reinterpret_cast<float *>(smem), *mine = merge + (size_t)warp * ROWS * (D + 2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -395,8 +463,8 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
         }
     __syncthreads();
     for (int i = tid; i < ROWS * (D / 2); i += THREADS) {
-        const int row = i / (D / 2), d = 2 * (i - row * (D / 2)), r = r0 + row;
-        if (r >= n_rows) break;
+        const int row = i / (D / 2), d = 2 * (i - row * (D / 2));
+        if (r0 + row >= n_rows) break;
         float M = -INFINITY, l = 0.f;
         float2 o = make_float2(0.f, 0.f);
 #pragma unroll
@@ -404,25 +472,53 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float *p = merge + ((size_t)w * ROWS + row) * (D + 2);
-            const float f = p[D] == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : exp2f(p[D] - M);         // (nothing seen: 0, or NaN, which stays one)
+            const float f = share_of(p[D], M);
             l += p[D + 1] * f;
             o.x += p[d] * f, o.y += p[d + 1] * f;
         }
-        const size_t tok = row0 + r / group, head = kvh * group + r % group;
+        const size_t tok = row0 + (r0 + row) / group, head = kvh * group + (r0 + row) % group;
         if (n_splits == 1) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<__nv_bfloat162 *>(out + tok * ldo + head * D + d) =
-                l == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o.x * inv, o.y * inv);
+            store_row(out + tok * ldo + head * D + d, o, l);
+        } else if (clustered) {
+            *reinterpret_cast<float2 *>(merge + (size_t)row * (D + 2) + d) = o;         // (no other thread reads it here)
+            if (d == 0) fin[row][0] = M, fin[row][1] = l;
         } else {
             const size_t at = (tok * H + head) * n_splits + split;
             *reinterpret_cast<float2 *>(part_o + at * D + d) = o;
             if (d == 0) part_ml[at] = make_float2(M, l);
         }
     }
+    if (!clustered) return;
+    // ---- the cluster's ranges together: each block joins a share of the results ----
+    __syncwarp();
+    cluster_sync();
+    for (int i = (int)block_of_cluster() * THREADS + tid; i < ROWS * (D / 2); i += n_splits * THREADS) {
+        const int row = i / (D / 2), d = 2 * (i - row * (D / 2));
+        if (r0 + row >= n_rows) break;
+        float2 ml[MAX_CLUSTER], part[MAX_CLUSTER];
+#pragma unroll
+        for (int j = 0; j < MAX_CLUSTER; ++j)
+            if (j < n_splits) ml[j] = load_there(fin[row], j), part[j] = load_there(merge + (size_t)row * (D + 2) + d, j);
+        float M = -INFINITY, l = 0.f;
+        float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < MAX_CLUSTER; ++j)
+            if (j < n_splits) M = fmaxf(M, ml[j].x);
+#pragma unroll
+        for (int j = 0; j < MAX_CLUSTER; ++j)
+            if (j < n_splits) {
+                const float f = share_of(ml[j].x, M);
+                l += ml[j].y * f;
+                o.x += part[j].x * f, o.y += part[j].y * f;
+            }
+        store_row(out + (size_t)(row0 + (r0 + row) / group) * ldo + (size_t)(kvh * group + (r0 + row) % group) * D + d, o, l);
+    }
+    __syncwarp();
+    cluster_sync();                         // (the others' shared memory is read until here)
 }
 
 // The ranges of one (token, head) in their order: a warp each.
-constexpr int JOIN_WARPS = 4;
+constexpr int JOIN_WARPS = 2;
 __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml,
                                                                     const int *__restrict__ seq_start, int limit, int n_tokens, __nv_bfloat16 *__restrict__ out,
                                                                     int ldo, int n_splits, int H, int D) {
@@ -433,47 +529,61 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const float 
     const int row0 = act_load(seq_start + s), n = act_load(seq_start + s + 1) - row0;
     if (j >= n || n > limit || head >= H || row0 < 0 || row0 + n > n_tokens) return;
     const size_t at = ((size_t)(row0 + j) * H + head) * n_splits;
-    float M = -INFINITY;
-    for (int i = lane; i < n_splits; i += 32) M = fmaxf(M, act_load(part_ml + at + i).x);
-    M = warp_max(M);
-    float l = 0.f;
-    float2 o[4] = {};
-    for (int i = 0; i < n_splits; ++i) {
-        const float2 ml = act_load(part_ml + at + i);
-        const float f = ml.x == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : exp2f(ml.x - M);
-        l += ml.y * f;
+    // lane i has the maxima and sums of ranges i, i + 32, ..; eight ranges' outputs are under way at a time
+    constexpr int PER_LANE = MAX_SPLITS / 32;
+    float2 ml[PER_LANE];
+    float M = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int d = 2 * (lane + 32 * u);
-            if (d < D) {
-                const float2 v = act_load(reinterpret_cast<const float2 *>(part_o + (at + i) * D + d));
-                o[u].x += v.x * f, o[u].y += v.y * f;
+    for (int p = 0; p < PER_LANE; ++p) {
+        ml[p] = lane + 32 * p < n_splits ? act_load(part_ml + at + lane + 32 * p) : make_float2(-INFINITY, 0.f);
+        M = fmaxf(M, ml[p].x);
+    }
+    M = warp_max(M);
+#pragma unroll
+    for (int p = 0; p < PER_LANE; ++p) {
+        ml[p].x = share_of(ml[p].x, M);
+        l += ml[p].y * ml[p].x;
+    }
+    l = warp_sum(l);
+    float2 o[2] = {};
+#pragma unroll
+    for (int p = 0; p < PER_LANE; ++p)
+        for (int i0 = 32 * p; i0 < min(n_splits, 32 * p + 32); i0 += 8) {
+            float2 v[8][2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int d = 2 * (lane + 32 * u);
+                    v[e][u] = i0 + e < n_splits && d < D ? act_load(reinterpret_cast<const float2 *>(part_o + (at + i0 + e) * D + d)) : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = __shfl_sync(0xffffffffu, ml[p].x, (i0 + e) & 31);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) o[u].x += v[e][u].x * f, o[u].y += v[e][u].y * f;
             }
         }
-    }
-    const float inv = 1.f / l;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < 2; ++u) {
         const int d = 2 * (lane + 32 * u);
-        if (d < D)
-            *reinterpret_cast<__nv_bfloat162 *>(out + (size_t)(row0 + j) * ldo + (size_t)head * D + d) =
-                l == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o[u].x * inv, o[u].y * inv);
+        if (d < D) store_row(out + (size_t)(row0 + j) * ldo + (size_t)head * D + d, o[u], l);
     }
 }
 
 template <int KS, int NT, bool Q8, typename... Args>
-int launch_one(dim3 grid, cudaStream_t stream, Args... args) {
-    const size_t smem = sizeof(float) * WARPS * 8 * NT * (KS * 16 + 2);
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<KS, NT, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) LGML_FAIL("tree_attention: cannot have %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    }
-    lgml_launch(tree_attention_kernel<KS, NT, Q8>, grid, THREADS, smem, stream, args...);
+int launch_one(dim3 grid, int cluster, cudaStream_t stream, Args... args) {
+    using C = Cut<KS, Q8>;
+    const size_t stages = (size_t)WARPS * C::STAGES * C::STAGE, merge = sizeof(float) * WARPS * 8 * NT * (KS * 16 + 2);
+    const size_t smem = stages > merge ? stages : merge;
+    cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<KS, NT, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) LGML_FAIL("tree_attention: cannot have %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    lgml_launch_cluster(tree_attention_kernel<KS, NT, Q8>, grid, THREADS, smem, stream, cluster, args...);
     return lgml_launch_status("tree_attention");
 }
 template <int KS, bool Q8, typename... Args>
 int launch_rows(int nt, Args... args) {
-    return nt == 1 ? launch_one<KS, 1, Q8>(args...) : launch_one<KS, 4, Q8>(args...);
+    return nt == 1 ? launch_one<KS, 1, Q8>(args...) : nt == 2 ? launch_one<KS, 2, Q8>(args...) : launch_one<KS, 4, Q8>(args...);
 }
 template <bool Q8, typename... Args>
 int launch_dim(int ks, Args... args) {
@@ -492,7 +602,7 @@ int launch_dim(int ks, Args... args) {
 }  // namespace
 
 LGML_API long long lgml_tree_attention_scratch_floats(int n_tokens, int H, int D, int n_splits) {
-    return n_splits <= 1 ? 0 : (long long)n_tokens * H * n_splits * (D + 2);
+    return n_splits <= MAX_CLUSTER ? 0 : (long long)n_tokens * H * n_splits * (D + 2);
 }
 
 // limit: requests that bring more tokens than this are left alone (their rows of out too).  k_exps null: pages in bfloat16.
@@ -506,26 +616,27 @@ LGML_API int lgml_tree_attention(const void *q, int ldq, const int *positions, c
     LGML_REQUIRE(D >= 16 && D <= 128 && D % 16 == 0, "tree_attention: head_dim %d must be a multiple of 16 up to 128", D);
     LGML_REQUIRE(limit >= 1 && limit <= MAX_NEW, "tree_attention: %d new tokens a request (1 to %d)", limit, MAX_NEW);
     LGML_REQUIRE(n_splits >= 1 && n_splits <= MAX_SPLITS, "tree_attention: %d key ranges (1 to %d)", n_splits, MAX_SPLITS);
-    LGML_REQUIRE(n_splits == 1 || (scratch != nullptr && ((uintptr_t)scratch & 7) == 0), "tree_attention: several ranges need scratch memory");
+    LGML_REQUIRE(n_splits <= MAX_CLUSTER || (scratch != nullptr && ((uintptr_t)scratch & 7) == 0), "tree_attention: several ranges need scratch memory");
     LGML_REQUIRE((k_exps == nullptr) == (v_exps == nullptr), "tree_attention: exponents for keys and values, or for neither");
-    LGML_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "tree_attention: the cache must be 16-byte aligned");
+    LGML_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_exps | (uintptr_t)v_exps) & 15) == 0, "tree_attention: the cache must be 16-byte aligned");
     LGML_REQUIRE(ldq % 2 == 0 && ((uintptr_t)q & 3) == 0 && ldo % 2 == 0 && ((uintptr_t)out & 3) == 0,
                  "tree_attention: q and out must be 4-byte aligned with even row strides");
-    LGML_REQUIRE((long long)n_seqs * limit <= 0x7fffffffLL, "tree_attention: too many requests");
+    LGML_REQUIRE((long long)n_seqs * (limit > n_splits ? limit : n_splits) <= 0x7fffffffLL, "tree_attention: too many requests");
     if (n_tokens == 0 || n_seqs == 0) return 0;
     const int rows = limit * (H / Hkv);
-    const int nt = rows <= 8 ? 1 : 4;
+    const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     const int n_chunks = (rows + 8 * nt - 1) / (8 * nt);
     LGML_REQUIRE((long long)Hkv * n_chunks <= 65535, "tree_attention: too many heads");
-    dim3 grid(n_seqs, Hkv * n_chunks, n_splits);
+    const int clustered = n_splits > 1 && n_splits <= MAX_CLUSTER;
+    dim3 grid(n_seqs * n_splits, Hkv * n_chunks);
     float *part_o = scratch;
-    float2 *part_ml = reinterpret_cast<float2 *>(scratch + (size_t)n_tokens * H * n_splits * D);
-#define LGML_ARGS D / 16, nt, grid, stream, (const __nv_bfloat16 *)q, ldq, positions, seq_start, seq_pos0, visible, block_table, max_blocks,            \
+    float2 *part_ml = scratch ? reinterpret_cast<float2 *>(scratch + (size_t)n_tokens * H * n_splits * D) : nullptr;
+#define LGML_ARGS D / 16, nt, grid, clustered ? n_splits : 1, stream, (const __nv_bfloat16 *)q, ldq, positions, seq_start, seq_pos0, visible, block_table, max_blocks,            \
                   (const uint8_t *)k_pages, (const uint8_t *)v_pages, (const uint8_t *)k_exps, (const uint8_t *)v_exps, n_pages, (__nv_bfloat16 *)out, ldo, \
-                  part_o, part_ml, n_splits, n_tokens, H, Hkv, n_chunks, limit, scale, window, status
+                  part_o, part_ml, n_splits, clustered, n_tokens, H, Hkv, n_chunks, limit, scale, window, status
     int rc = k_exps ? launch_dim<true>(LGML_ARGS) : launch_dim<false>(LGML_ARGS);
 #undef LGML_ARGS
-    if (rc || n_splits == 1) return rc;
+    if (rc || n_splits <= MAX_CLUSTER) return rc;
     lgml_launch(tree_join_kernel, dim3(n_seqs * limit, (H + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, part_o, part_ml, seq_start, limit,
                 n_tokens, (__nv_bfloat16 *)out, ldo, n_splits, H, D);
     return lgml_launch_status("tree_attention_join");

@@ -22,7 +22,6 @@ namespace {
 constexpr int PAGE = 64;
 constexpr int WARPS = 8;
 constexpr int MAX_D = 256;
-constexpr int PAIRS = MAX_D / 64;        // pairs of entries a lane holds at most
 constexpr int LOWEST = -60, HIGHEST = 119;
 
 // The exponent of a vector whose largest finite entry is amax: 448 = 1.75 x 2^8.
@@ -42,9 +41,9 @@ __device__ __forceinline__ unsigned short e4m3_pair(float a, float b, float inv)
     return r;
 }
 
-// A warp a head of a token; a lane holds pairs lane, lane + 32, .. of the head, so the vector's largest entry is one warp
-// reduction.  pairing and the treatment of entries past n_rot as in rope_cache.cu.
-template <typename TS, bool Q8>
+// Few tokens, and any head size: a warp a head of a token; a lane holds pairs lane, lane + 32, .. (PAIRS at most) of the head, so the vector's
+// largest entry is one warp reduction.  pairing and the treatment of entries past n_rot as in rope_cache.cu.
+template <typename TS, bool Q8, int PAIRS>
 __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
     const TS *__restrict__ src, int lds, int n_parts, long long part_stride, const float *__restrict__ bias, __nv_bfloat16 *__restrict__ q_out, int ldq,
     const int *__restrict__ positions, const int *__restrict__ cells, const int *__restrict__ seq_of_token, const int *__restrict__ block_table,
@@ -142,6 +141,102 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
     }
 }
 
+// The same for many tokens, bfloat16 in, heads of 64 or 128 entries that turn whole: a block a token, whose angles are computed once for all its
+// heads; sixteen lanes a head, each with P = D / 32 neighbouring entries of the first half of the head and P of the second ("half"), or 2 P
+// neighbouring entries ("adjacent"): either way the pairs that turn together are in one thread, and loads and stores are 4 P and 2 P bytes wide.
+constexpr int WIDE_THREADS = 256, WIDE_FROM = 24;
+template <int P> struct Vec;
+template <> struct Vec<2> { using type = unsigned; };
+template <> struct Vec<4> { using type = uint2; };
+template <> struct Vec<8> { using type = uint4; };
+template <int P, bool Q8, bool ADJACENT>
+__global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
+    const __nv_bfloat16 *__restrict__ src, int lds, __nv_bfloat16 *__restrict__ q_out, int ldq, const int *__restrict__ positions, const int *__restrict__ cells,
+    const int *__restrict__ seq_of_token, const int *__restrict__ block_table, int n_seqs, int max_blocks, const float *__restrict__ inv_freq,
+    const float *__restrict__ inv_freq_lo, void *__restrict__ k_pages, void *__restrict__ v_pages, uint8_t *__restrict__ k_exps, uint8_t *__restrict__ v_exps,
+    int n_pages, int H, int Hkv, int n_heads, int *__restrict__ status) {
+    pdl_trigger();
+    constexpr int D = 32 * P;
+    using Half = typename Vec<P>::type;
+    __shared__ float2 turn[D / 2];           // (cos, sin) of pair i
+    const int t = blockIdx.x, tid = threadIdx.x, l = tid & 15;
+    const int pos = early_int(positions + t), cell = cells ? early_int(cells + t) : pos, seq = early_int(seq_of_token + t), blk = cell / PAGE;
+    const int page = cell >= 0 && blk < max_blocks && seq >= 0 && seq < n_seqs ? early_int(block_table + (size_t)seq * max_blocks + blk) : -1;
+    if (tid < D / 2) {
+        float sn, cs;
+        rope_sincos(pos, early_weight(inv_freq + tid), inv_freq_lo ? early_weight(inv_freq_lo + tid) : 0.f, &sn, &cs);
+        turn[tid] = make_float2(cs, sn);
+    }
+    const bool there = page >= 0 && page < n_pages;
+    if (!there && n_heads > H && tid == 0) atomicExch(status, 2);      // the host reserves pages first; never write outside the pool
+    __syncthreads();
+    pdl_wait();
+    // entries e of the first run and of the second; pair i of the thread is (x[i], x[P + i]) or, adjacent, (x[2 i], x[2 i + 1])
+    const int run0 = ADJACENT ? 2 * P * l : P * l, run1 = ADJACENT ? run0 + P : run0 + D / 2;
+    constexpr int UNITS = WIDE_THREADS / 16;
+    for (int base = 0; base < n_heads; base += 2 * UNITS) {       // (both heads of a warp go round as often)
+        const int head = base + tid / 16;
+        Half raw[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (head + k * UNITS < n_heads) {
+                const __nv_bfloat16 *p = src + (size_t)t * lds + (size_t)(head + k * UNITS) * D;
+                raw[k][0] = __ldcg(reinterpret_cast<const Half *>(p + run0)), raw[k][1] = __ldcg(reinterpret_cast<const Half *>(p + run1));
+            }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int h = head + k * UNITS;
+            const bool mine = h < n_heads;              // (the lanes of a head are together in this, and in the reduction below)
+            float x[2 * P];
+#pragma unroll
+            for (int i = 0; i < 2 * P; ++i) x[i] = mine ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(raw[k])[i]) : 0.f;
+            if (h < H + Hkv) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int a = ADJACENT ? 2 * i : i, b = ADJACENT ? 2 * i + 1 : P + i;
+                    const float2 f = turn[P * l + i];
+                    const float u = x[a] * f.x - x[b] * f.y, v = x[a] * f.y + x[b] * f.x;
+                    x[a] = u, x[b] = v;
+                }
+            }
+            const size_t vec = there ? ((size_t)page * Hkv + (h < H + Hkv ? h - H : h - H - Hkv)) * PAGE + cell % PAGE : 0;
+            if (Q8) {
+                float amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * P; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                if (mine && h >= H && there) {
+                    const int e = vector_exponent(amax);
+                    const float inv = power_of_two(-e);
+                    unsigned short c[P];
+#pragma unroll
+                    for (int i = 0; i < P; ++i) c[i] = e4m3_pair(x[2 * i], x[2 * i + 1], inv);
+                    uint8_t *dst = reinterpret_cast<uint8_t *>(h < H + Hkv ? k_pages : v_pages) + vec * D;
+                    if (ADJACENT) {
+                        if (P == 4) *reinterpret_cast<uint2 *>(dst + run0) = make_uint2(c[0] | (unsigned)c[1 % P] << 16, c[2 % P] | (unsigned)c[3 % P] << 16);
+                        else *reinterpret_cast<unsigned *>(dst + run0) = c[0] | (unsigned)c[1] << 16;
+                    } else if (P == 4) {
+                        *reinterpret_cast<unsigned *>(dst + run0) = c[0] | (unsigned)c[1 % P] << 16;
+                        *reinterpret_cast<unsigned *>(dst + run1) = c[2 % P] | (unsigned)c[3 % P] << 16;
+                    } else {
+                        *reinterpret_cast<unsigned short *>(dst + run0) = c[0];
+                        *reinterpret_cast<unsigned short *>(dst + run1) = c[1];
+                    }
+                    if (l == 0) (h < H + Hkv ? k_exps : v_exps)[vec] = (uint8_t)(e + 127);
+                }
+            }
+            if (!mine || (h >= H && (Q8 || !there))) continue;
+            __nv_bfloat16 *dst = h < H ? q_out + (size_t)t * ldq + (size_t)h * D : reinterpret_cast<__nv_bfloat16 *>(h < H + Hkv ? k_pages : v_pages) + vec * D;
+            Half y[2];
+#pragma unroll
+            for (int i = 0; i < P; ++i) reinterpret_cast<__nv_bfloat162 *>(y)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            *reinterpret_cast<Half *>(dst + run0) = y[0];
+            *reinterpret_cast<Half *>(dst + run1) = y[1];
+        }
+    }
+}
+
 // Page list[i] of the pool as bfloat16 page i of the output: a block per (page, KV head, keys or values), 16 codes a thread and turn.
 // An entry below zero leaves its page of the output as it is; one past the pool does too, and sets the status.
 constexpr int READ_THREADS = 128;
@@ -183,8 +278,18 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_kernel(const uint8_t *__
 }
 
 template <typename TS, bool Q8, typename... Args>
-int launch_store(dim3 grid, cudaStream_t stream, const void *src, Args... args) {
-    lgml_launch(kv_store_kernel<TS, Q8>, grid, WARPS * 32, 0, stream, (const TS *)src, args...);
+int launch_store(int D, dim3 grid, cudaStream_t stream, const void *src, Args... args) {
+    if (D <= 64) lgml_launch(kv_store_kernel<TS, Q8, 1>, grid, WARPS * 32, 0, stream, (const TS *)src, args...);
+    else if (D <= 128) lgml_launch(kv_store_kernel<TS, Q8, 2>, grid, WARPS * 32, 0, stream, (const TS *)src, args...);
+    else lgml_launch(kv_store_kernel<TS, Q8, 4>, grid, WARPS * 32, 0, stream, (const TS *)src, args...);
+    return lgml_launch_status("rope_kv_store");
+}
+template <int P, typename... Args>
+int launch_wide(bool q8, bool adjacent, int n_tokens, cudaStream_t stream, Args... args) {
+    if (q8 && adjacent) lgml_launch(kv_store_wide_kernel<P, true, true>, dim3(n_tokens), WIDE_THREADS, 0, stream, args...);
+    else if (q8) lgml_launch(kv_store_wide_kernel<P, true, false>, dim3(n_tokens), WIDE_THREADS, 0, stream, args...);
+    else if (adjacent) lgml_launch(kv_store_wide_kernel<P, false, true>, dim3(n_tokens), WIDE_THREADS, 0, stream, args...);
+    else lgml_launch(kv_store_wide_kernel<P, false, false>, dim3(n_tokens), WIDE_THREADS, 0, stream, args...);
     return lgml_launch_status("rope_kv_store");
 }
 }  // namespace
@@ -203,8 +308,16 @@ LGML_API int lgml_rope_kv_store(const void *src, int src_type, int lds, int n_pa
     if (n_tokens == 0) return 0;
     const int n_heads = write_kv ? H + 2 * Hkv : H;
     LGML_REQUIRE((n_heads + WARPS - 1) / WARPS <= 65535, "rope_kv_store: too many heads");
+    // many tokens whose heads turn whole, everything on the width of a thread's loads and stores
+    if (src_type == LGML_BF16 && n_tokens >= WIDE_FROM && n_rot == D && (D == 64 || D == 128) && lds % 8 == 0 && ldq % 8 == 0 &&
+        (((uintptr_t)src | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0) {
+#define LGML_ARGS k_exps != nullptr, pairing != 0, n_tokens, stream, (const __nv_bfloat16 *)src, lds, (__nv_bfloat16 *)q_out, ldq, positions, cells, seq_of_token, \
+                  block_table, n_seqs, max_blocks, inv_freq, inv_freq_lo, k_pages, v_pages, (uint8_t *)k_exps, (uint8_t *)v_exps, n_pages, H, Hkv, n_heads, status
+        return D == 64 ? launch_wide<2>(LGML_ARGS) : launch_wide<4>(LGML_ARGS);
+#undef LGML_ARGS
+    }
     dim3 grid(n_tokens, (n_heads + WARPS - 1) / WARPS);
-#define LGML_ARGS grid, stream, src, lds, n_parts, part_stride, bias, (__nv_bfloat16 *)q_out, ldq, positions, cells, seq_of_token, block_table, n_seqs,  \
+#define LGML_ARGS D, grid, stream, src, lds, n_parts, part_stride, bias, (__nv_bfloat16 *)q_out, ldq, positions, cells, seq_of_token, block_table, n_seqs,  \
                   max_blocks, inv_freq, inv_freq_lo, n_rot, pairing, k_pages, v_pages, (uint8_t *)k_exps, (uint8_t *)v_exps, n_pages, H, Hkv, D, n_heads, \
                   status
     if (src_type == LGML_F32) return k_exps ? launch_store<float, true>(LGML_ARGS) : launch_store<float, false>(LGML_ARGS);

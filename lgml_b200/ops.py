@@ -2932,6 +2932,7 @@ def paged_attention(q, batch, cache, out, n_heads: int, scale: float, window: in
 E4M3 = torch.float8_e4m3fn
 TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
 TREE_MAX_DIM = 128
+TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
 
 
@@ -3081,7 +3082,7 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
 
 def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64) -> int:
     """Into how many ranges of pages ``tree_attention`` cuts a request's cells."""
-    blocks = max(n_seqs * n_kv_heads * -(-rows // (8 if rows <= 8 else 32)), 1)
+    blocks = max(n_seqs * n_kv_heads * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32)), 1)
     pages = max(1, -(-longest // page))
     return max(1, min(-(-pages // 2), (4 * sm_count()) // blocks, 64))
 
@@ -3119,7 +3120,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
             raise KernelError(f"{who}: one mask a token")
     if n_splits is None:
         n_splits = tree_splits(seqs, hkv, max_new_tokens * (n_heads // hkv), max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page))
-    if n_splits > 1:
+    if n_splits > TREE_CLUSTER:
         need = n * n_heads * n_splits * (d + 2)
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -3131,7 +3132,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
                                                        c_void_p, c_void_p])
     _check("attention_tree", fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
                                 blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
-                                scratch.data_ptr() if n_splits > 1 else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
+                                scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
                                 status.data_ptr(), _stream()), who)
     return out
 

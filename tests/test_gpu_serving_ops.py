@@ -81,7 +81,8 @@ def turned(x, positions, exact, n_rot, pairing):
 @pytest.mark.parametrize("H,G,D,n_rot,pairing,parts,bias", [
     (4, 2, 16, 16, "half", 0, False), (6, 2, 32, 32, "adjacent", 3, True), (5, 5, 48, 24, "half", 1, False), (8, 2, 64, 64, "half", 9, True),
     (3, 1, 80, 0, "half", 0, False), (4, 4, 96, 96, "adjacent", 0, False), (2, 1, 112, 2, "adjacent", 2, False), (32, 8, 128, 128, "half", 4, False),
-    (2, 2, 256, 128, "half", 0, False), (7, 1, 128, 128, "adjacent", 0, False)])
+    (2, 2, 256, 128, "half", 0, False), (7, 1, 128, 128, "adjacent", 0, False),
+    (8, 2, 64, 64, "half", 0, False), (5, 2, 64, 64, "adjacent", 0, False), (17, 4, 128, 128, "half", 0, False), (32, 8, 128, 64, "half", 0, False)])
 def test_store_writes_cells_and_turns_by_positions(H, G, D, n_rot, pairing, parts, bias, eight):
     from lgml_b200 import ops
 
@@ -338,7 +339,7 @@ def test_attention_of_one_token_at_every_head_size(H, G, D, eight):
 @pytest.mark.parametrize("H,G,D", [(8, 2, 64), (32, 8, 128), (6, 2, 32)])
 def test_attention_of_chains_and_trees(H, G, D, lens, pos0, tree, eight):
     p = Problem(lens, pos0, H, G, D, eight, tree=tree, seed=len(lens))
-    for n_splits in (None, 1, 7):
+    for n_splits in (None, 1, 7, 12):
         p.check(p.run(n_splits=n_splits))
 
 
@@ -569,7 +570,7 @@ def test_refusals():
                dict(table=ints(p.table).cpu()), dict(cells=ints([1, 2])), dict(q_out=torch.zeros(3, 512, device=DEV))):
         with pytest.raises(ops.KernelError):
             store(**kw)
-    for kw in (dict(most=65), dict(q=p.q[:, :-64]), dict(q=p.q.float()), dict(n_splits=257), dict(n_splits=0), dict(n_splits=2, scratch=torch.zeros(8, device=DEV)),
+    for kw in (dict(most=65), dict(q=p.q[:, :-64]), dict(q=p.q.float()), dict(n_splits=257), dict(n_splits=0), dict(n_splits=9, scratch=torch.zeros(8, device=DEV)),
                dict(out=torch.zeros(3, 512, device=DEV))):
         with pytest.raises(ops.KernelError):
             p.run(**kw)
