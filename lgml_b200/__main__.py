@@ -25,6 +25,8 @@ def main(argv=None) -> int:
     ap.add_argument("-np", "--parallel", type=int, default=4, help="slots: the most requests kept at once (default 4)")
     ap.add_argument("-ub", "--ubatch", type=int, default=512, help="prompt tokens per request per pass (default 512)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", choices=["bfloat16", "float32", "float8_e4m3"], help="type of the cache's keys and values (default: --dtype; float8_e4m3: eight bits)")
+    ap.add_argument("--logprobs", type=int, metavar="K", help="print, to standard error, every new token's log probability, rank and entropy with the K most probable tokens")
     ap.add_argument("--prefix-cache", action="store_true", help="keep the full pages of ended requests findable: a prompt that begins like an earlier one computes only the rest")
     ap.add_argument("--prompt-ids", action="append", default=[], help="comma-separated token ids; repeat for more requests")
     ap.add_argument("-n", "--max-tokens", type=int, default=16, help="new tokens per request")
@@ -58,7 +60,7 @@ def main(argv=None) -> int:
         ap.error("give at least one --prompt-ids")
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in args.prompt_ids]
     eng = Engine(args.model, config=cfg, random_weights=args.seed or 0, dtype=args.dtype, n_ctx=args.ctx, slots=args.parallel,
-                 ubatch=args.ubatch, repeat_stop_tokens=args.repeat_stop, prefix_cache=args.prefix_cache)
+                 ubatch=args.ubatch, repeat_stop_tokens=args.repeat_stop, prefix_cache=args.prefix_cache, cache_dtype=args.cache_dtype)
     import contextlib
 
     from . import ops
@@ -67,7 +69,7 @@ def main(argv=None) -> int:
         outs = eng.generate(prompts, max_tokens=args.max_tokens, seed=args.seed, temperature=args.temperature, top_k=args.top_k,
                             top_p=args.top_p, min_p=args.min_p, repeat_penalty=args.repeat_penalty,
                             frequency_penalty=args.frequency_penalty, presence_penalty=args.presence_penalty,
-                            repeat_last_n=args.repeat_last_n,
+                            repeat_last_n=args.repeat_last_n, logprobs=args.logprobs,
                             on_token=(lambda i, t: print(f"{i}: {t}", flush=True)) if args.stream else None)
     if kt is not None:
         tot = kt.totals()
@@ -75,6 +77,11 @@ def main(argv=None) -> int:
             print(f"{name:28s} {tot[name]:12.1f} us in {tot[name + ' calls']} calls", file=sys.stderr)
     if args.turn_csv:
         eng.write_turn_csv(args.turn_csv)
+    if args.logprobs is not None:
+        for i, (_, scores) in enumerate(outs):
+            for sc in scores:
+                print(f"{i}: {sc.id} logprob {sc.logprob:.6f} rank {sc.rank} entropy {sc.entropy:.6f} top {' '.join(f'{t}:{lp:.6f}' for t, lp in sc.top)}", file=sys.stderr)
+        outs = [ids for ids, _ in outs]
     for o in outs:
         print(",".join(str(t) for t in o))
     return 0

@@ -25,6 +25,9 @@ last token is always computed, since its logits are wanted.  Shared pages are on
 a request writes behind its prefix, into pages of its own.  This needs every layer to keep
 all its keys (no window, no state of fixed size: those cannot be taken up in the middle,
 ``check_pass`` ``lua/lgml/transformer.lua:1548-1563``).
+
+``page_dtype`` ``torch.float8_e4m3fn`` keeps keys and values in eight bits (the reference's quantised cache types,
+``lua/lgml/kv.lua:14-17``, have the same purpose): half the pages' bytes, and one byte a vector for its power of two.
 """
 from __future__ import annotations
 
@@ -67,6 +70,10 @@ class FixedState:
     dtype: torch.dtype = torch.float32
 
 
+# Pages of eight bits: e4m3 codes, and a byte a vector for its power of two (``ops.rope_kv_store``).
+EIGHT_BIT = torch.float8_e4m3fn
+
+
 class NoSlot(RuntimeError):
     """Every request slot is taken."""
 
@@ -78,6 +85,8 @@ class PagedGroup:
     pool: PagePool
     k: Dict[int, torch.Tensor] = field(default_factory=dict)  # layer -> [n_pages, Hkv, page, D]
     v: Dict[int, torch.Tensor] = field(default_factory=dict)
+    k_exps: Dict[int, torch.Tensor] = field(default_factory=dict)  # layer -> uint8 [n_pages, Hkv, page], in a cache of eight bits
+    v_exps: Dict[int, torch.Tensor] = field(default_factory=dict)
 
 
 @dataclass
@@ -108,7 +117,7 @@ class CacheManager:
     """
 
     def __init__(self, layout: Dict[int, object], n_pages: int, max_slots: int, dtype: torch.dtype, device,
-                 page_size: int = PAGE_SIZE, max_step_tokens: int = 0, prefix_cache: bool = False):
+                 page_size: int = PAGE_SIZE, max_step_tokens: int = 0, prefix_cache: bool = False, page_dtype: Optional[torch.dtype] = None):
         if max_slots <= 0:
             raise ValueError("max_slots must be positive")
         self.prefix_cache = bool(prefix_cache)
@@ -116,6 +125,7 @@ class CacheManager:
         self.max_slots = max_slots
         self.device = torch.device(device)
         self.dtype = dtype
+        self.page_dtype = page_dtype if page_dtype is not None else dtype
         self.groups: List[PagedGroup] = []
         self.state_groups: List[StateGroup] = []
         self.group_of_layer: Dict[int, int] = {}
@@ -157,6 +167,13 @@ class CacheManager:
             v_shape = (shape[0], grp.spec.v_heads or grp.spec.n_kv_heads, page_size, v_dim)
             if grp.spec.v_in_k and (v_dim > grp.spec.head_dim or v_shape[1] != grp.spec.n_kv_heads):
                 raise ValueError(f"values inside the key cells need the keys' head count and at most their size: {grp.spec}")
+            if self.page_dtype == EIGHT_BIT:
+                if grp.spec.v_in_k or v_shape != shape:
+                    raise ValueError(f"a cache of eight bits keeps keys and values of one shape, each its own: {grp.spec}")
+                for layer in grp.layers:
+                    grp.k[layer], grp.v[layer] = [torch.zeros(shape, dtype=torch.uint8, device=self.device).view(EIGHT_BIT) for _ in range(2)]
+                    grp.k_exps[layer], grp.v_exps[layer] = [torch.zeros(shape[:3], dtype=torch.uint8, device=self.device) for _ in range(2)]
+                continue
             for layer in grp.layers:
                 grp.k[layer] = torch.zeros(shape, dtype=dtype, device=self.device)
                 grp.v[layer] = grp.k[layer][..., :v_dim] if grp.spec.v_in_k else torch.zeros(v_shape, dtype=dtype, device=self.device)
@@ -189,6 +206,7 @@ class CacheManager:
             n += sum(t.numel() * t.element_size() for t in g.k.values())
             if not g.spec.v_in_k:
                 n += sum(t.numel() * t.element_size() for t in g.v.values())
+            n += sum(t.numel() for exps in (g.k_exps, g.v_exps) for t in exps.values())
         for sg in self.state_groups:
             n += sum(t.numel() * t.element_size() for t in sg.state.values())
         return n

@@ -37,6 +37,9 @@ class CacheView:
     writable: bool = True
     state: Optional[torch.Tensor] = None        # [max_slots, ...] for a fixed-state layer
     page_size: int = 0
+    k_exps: Optional[torch.Tensor] = None       # uint8 [pages, Hkv, page]: the vectors' powers of two, in a cache of eight bits
+    v_exps: Optional[torch.Tensor] = None
+    group: int = 0                              # which of the cache's groups of layers
 
 
 def cache_view_of(cm, owner: int, block_tables, writable: bool = True) -> CacheView:
@@ -46,7 +49,8 @@ def cache_view_of(cm, owner: int, block_tables, writable: bool = True) -> CacheV
     g = cm.group_of_layer.get(owner)
     if g is not None:
         grp = cm.groups[g]
-        view = CacheView(k=grp.k[owner], v=grp.v[owner], block_table=block_tables[g], writable=writable, page_size=cm.page_size)
+        view = CacheView(k=grp.k[owner], v=grp.v[owner], block_table=block_tables[g], writable=writable, page_size=cm.page_size,
+                         k_exps=grp.k_exps.get(owner), v_exps=grp.v_exps.get(owner), group=g)
     sg = cm.state_group_of_layer.get(owner)
     if sg is not None:
         view.state = cm.state_groups[sg].state[owner]
@@ -96,6 +100,8 @@ class StepBatch:
         self.min_kv_len = min(self.kv_lens) if lens else 0
         self.decode_splits = None       # a fixed split count (set by a captured graph)
         self.shared = {}                # what one layer of this step keeps for later layers (by name)
+        self.cells = None               # where the tokens' keys lie (None: at their positions) and what each sees of its request's new tokens
+        self.visible = None             # (``tree``): int32 [N] and int64 [N] on the device
         self._tiles = {}
         self.replayed = False           # are its launches recorded, and run again for other contexts?
         self.replay_reach = 0           # ... of over half of so many tokens and up to all of them (0: any that are short)
@@ -268,6 +274,39 @@ class StepBatch:
             else:
                 cached = (self.attention_tiles(tile_tokens, up_to if rows.size else 0, remember=False), self._to_device(rows.astype(np.int32)) if rows.size else None, longest)
             self._tiles[key] = cached
+        return cached
+
+    def tree(self, parents: Sequence[Sequence[int]]) -> None:
+        """Every request's tokens form a tree: ``parents[s][i]`` is the place, before i, of the token that i follows (-1: it follows what the
+        request has in the cache).  A token's position is then what its request holds plus its depth; its key lies where it would
+        in a chain; and it sees what is in the cache, its forebears and itself."""
+        depth, masks = [], []
+        for pos0, ps in zip(self.pos0, parents):
+            d, m = [], []
+            for i, p in enumerate(ps):
+                d.append(0 if p < 0 else d[p] + 1)
+                m.append((0 if p < 0 else m[p]) | 1 << i)
+            depth += [pos0 + x for x in d]
+            masks += m
+        dev = self.token_ids.device
+        self.cells = self.positions
+        self.positions = torch.tensor(depth, dtype=torch.int32).to(dev)
+        self.visible = torch.from_numpy(np.array(masks, dtype=np.uint64).view(np.int64)).to(dev)
+
+    def read_back(self, group: int, longer_than: int):
+        """For attention that takes pages of bfloat16 over a cache of eight bits: the pages of the requests that bring more than ``longer_than`` tokens
+        (int32 [n], each once) and a block table [requests, width] whose entries are places in that list.  Made once per step and group."""
+        key = ("read back", group, longer_than)
+        cached = self._tiles.get(key)
+        if cached is None:
+            place: Dict[int, int] = {}
+            table = np.full((self.n_seqs, self.table_width[group]), -1, dtype=np.int32)
+            for s, (req, n) in enumerate(zip(self.requests, self.seq_lens)):
+                if n > longer_than:
+                    row = req.tables[group]
+                    table[s, :len(row)] = [place.setdefault(p, len(place)) if p >= 0 else -1 for p in row]
+            pages = np.fromiter(place, dtype=np.int32, count=len(place))
+            cached = self._tiles[key] = (self._to_device(pages), self._to_device(table.reshape(-1)).view(self.n_seqs, -1))
         return cached
 
     def _to_device(self, arr: np.ndarray) -> torch.Tensor:

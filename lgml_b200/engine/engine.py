@@ -12,8 +12,10 @@ default 512), ``max_tokens`` (default reply length: the free context),
 the host has seen the ids of the one before, when those are chosen on the device.
 ``prefix_cache`` (always on in the reference, ``E:reuse`` ``lua/lgml/engine.lua:1775-1819``; off by default
 here): the full pages of ended and preempted requests stay findable by a key of their tokens, and a
-prompt that begins like one of them computes only the rest.  ``generate.greedy`` of the reference
-(``lua/lgml/generate.lua:19-34``) is ``Engine.greedy``.
+prompt that begins like one of them computes only the rest.  ``cache_dtype`` ("float8_e4m3": keys and values in
+eight bits, half the cache's bytes; the reference's quantised cache types, ``lua/lgml/kv.lua:14-17``).  ``Engine.score``: log
+probabilities of given tokens; ``generate(logprobs=k)``: of the generated ones.  ``generate.greedy`` of the reference
+(``lua/lgml/generate.lua:19-34``) is ``Engine.greedy``, which can check drafted tokens (``draft``).
 """
 from __future__ import annotations
 
@@ -28,11 +30,25 @@ from ..cache import PAGE_SIZE
 from ..sampling import Sampler, SamplingParams, log_min_p
 from .runner import ModelRunner
 from .runtime import MAX_RESULT
+from .scores import PendingScores, TokenScore
 from .scheduler import REPEAT_STOP, UBATCH, GenRequest, Scheduler
 
 DEFAULT_CTX = 4096      # context of a model whose configuration names no limit of positions, when none is given
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32, "f32": torch.float32}
+
+
+_CACHE_DTYPES = {**_DTYPES, "float8_e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+
+
+def parse_cache_dtype(name) -> Optional[torch.dtype]:
+    """The type of the cache's pages (None: the compute type)."""
+    if name is None or isinstance(name, torch.dtype):
+        return name
+    try:
+        return _CACHE_DTYPES[str(name)]
+    except KeyError:
+        raise ValueError(f"unknown cache type '{name}' (known: {', '.join(sorted(_CACHE_DTYPES))})") from None
 
 
 def parse_dtype(name) -> torch.dtype:
@@ -48,7 +64,7 @@ class Engine:
     def __init__(self, model=None, *, config=None, random_weights: Optional[int] = None, dtype="bfloat16", n_ctx: Optional[int] = None,
                  kv_tokens: Optional[int] = None, slots: int = 4, ubatch: int = UBATCH, max_batch_tokens: Optional[int] = None, max_tokens: Optional[int] = None,
                  sampling: Optional[dict] = None, repeat_stop_tokens: int = REPEAT_STOP, device="cuda:0",
-                 run_ahead: bool = True, prefix_cache: bool = False):
+                 run_ahead: bool = True, prefix_cache: bool = False, cache_dtype=None):
         dt = parse_dtype(dtype)
         if model is None and config is None:
             raise ValueError("give a model folder, or a config with random_weights=seed")
@@ -68,7 +84,8 @@ class Engine:
         # the pool all slots share: n_ctx tokens as in the reference, or kv_tokens when given
         n_pages = -(-(kv_tokens or n_ctx) // PAGE_SIZE)
         max_batch_tokens = max_batch_tokens or max(ubatch, 2048)
-        kw = dict(n_pages=n_pages, max_slots=slots, max_step_tokens=max_batch_tokens, prefix_cache=prefix_cache)
+        kw = dict(n_pages=n_pages, max_slots=slots, max_step_tokens=max_batch_tokens, prefix_cache=prefix_cache,
+                  cache_dtype=parse_cache_dtype(cache_dtype))
         if model is not None:
             self.runner = ModelRunner.from_folder(model, dt, device, **kw)
         else:
@@ -87,6 +104,7 @@ class Engine:
         gc.freeze()
         self._next_id = 0
         self._on_token = None
+        self._logprobs: Optional[int] = None        # alternatives per generated token whose scores ``generate`` was asked for
         self.run_ahead = run_ahead
         self._ahead: Optional[dict] = None          # the step whose ids the host has not seen yet
         self._host_ring = [torch.empty(MAX_RESULT + 1, dtype=torch.int32).pin_memory() for _ in range(3)]
@@ -151,6 +169,9 @@ class Engine:
         else:
             host_logits = logits.cpu().numpy()
             rec["toks"] = [int(e.request.sampler.sample(host_logits[i])) for i, e in enumerate(rows)]
+        if self._logprobs is not None:
+            ids = rec["out"] if rec["toks"] is None else torch.tensor(rec["toks"], dtype=torch.int32).to(logits.device)
+            rec["scores"] = PendingScores(logits, ids, self._logprobs, self.rt.status)
         return rec
 
     def _ids_to_host(self, rec: dict, out: torch.Tensor) -> None:
@@ -214,6 +235,11 @@ class Engine:
         # a request that an earlier step ended has a token too many in this one: not counted
         n_decode = sum(1 for e in plan if len(e.tokens) == 1 and e.sample and e.request.finish_reason is None)
         done = self.scheduler.complete(plan, {e.request.id: int(t) for e, t in zip(rows, toks)})
+        if "scores" in rec:
+            for e, t, score in zip(rows, toks, rec["scores"].scores(toks)):
+                r = e.request
+                if len(r.scores) < len(r.generated):        # (a token too many was dropped by ``complete``)
+                    r.scores.append(score)
         if self._on_token is not None:
             # (a token too many, run ahead of the end token that finished its request, was dropped by ``complete``)
             for e, t in zip(rows, toks):
@@ -273,7 +299,7 @@ class Engine:
     # ---- public --------------------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: Optional[int] = None, stop: Optional[Sequence[int]] = None,
                  seed: Optional[int] = None, return_details: bool = False, per_prompt: Optional[Sequence[dict]] = None,
-                 on_token=None, **sampling):
+                 on_token=None, logprobs: Optional[int] = None, **sampling):
         """Token ids in, token ids out.  ``prompts``: lists of token ids.  Sampler options
         (``temperature``, ``top_k``, ``top_p``, ``min_p``, ``repeat_penalty``,
         ``frequency_penalty``, ``presence_penalty``, ``repeat_last_n``, ``logit_bias``) and
@@ -281,7 +307,13 @@ class Engine:
         ``per_prompt``: one dict of sampler options per prompt that override the common ones.
         ``on_token(i, id)`` is called for every new token of prompt i as soon as the host knows it
         (the reference streams its replies the same way).
+        ``logprobs`` = k: every new token's ``TokenScore`` with the k most probable ones (k up to 32), of the distribution that the logits gave after
+        ``logit_bias`` and the penalties, before temperature and truncation; the result is then (ids, scores) per prompt (``GenRequest.scores`` with
+        ``return_details``).
         Returns one list of new ids per prompt (with the stop id when one ends it)."""
+        if logprobs is not None and not 0 <= logprobs <= min(ops.LOGPROBS_TOP, self.runner.model.vocab_size):
+            raise ValueError(f"logprobs: {logprobs} alternatives (0 to {min(ops.LOGPROBS_TOP, self.runner.model.vocab_size)})")
+        self._logprobs = logprobs
         opts = {**self.sampling_defaults, **sampling}
         stop_ids = list(stop) if stop is not None else self.eos_ids
         reqs = []
@@ -296,6 +328,8 @@ class Engine:
             req = GenRequest(id=("gen", self._next_id), prompt=p, max_new_tokens=max(min(limit, room), 0), params=params,
                              stop_ids=stop_ids)
             req.index, req._told = i, 0
+            if logprobs is not None:
+                req.scores = []
             self._next_id += 1
             if req.max_new_tokens == 0:
                 req.finish_reason = "length"
@@ -308,17 +342,50 @@ class Engine:
         self.timings = {"total": time.perf_counter() - t0}
         if return_details:
             return reqs
+        if logprobs is not None:
+            return [(r.generated, r.scores) for r in reqs]
         return [r.generated for r in reqs]
 
-    def greedy(self, prompt: Sequence[int], n_predict: int, stop: Optional[Sequence[int]] = None):
-        """Greedy decode of one prompt: (new ids, timings {prefill, decode, n_decode}), as
-        ``generate.greedy`` (``lua/lgml/generate.lua:19-34``)."""
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
+        """The log probability of every given token but the first behind those before it, with rank, entropy and the ``top`` (up to 32) most probable
+        tokens: one list of ``TokenScore`` per prompt, one shorter than it."""
+        runner = self.runner
+        vocab = runner.model.vocab_size
+        prompts = [[int(t) for t in p] for p in prompts]
+        if not 0 <= top <= min(ops.LOGPROBS_TOP, vocab):
+            raise ValueError(f"score: {top} alternatives (0 to {min(ops.LOGPROBS_TOP, vocab)})")
+        for i, p in enumerate(prompts):
+            if not p or len(p) > self.n_ctx or not all(0 <= t < vocab for t in p):
+                raise ValueError(f"score: prompt {i} must have 1 to {self.n_ctx} tokens of the vocabulary")
+        out: List[List[TokenScore]] = []
+        for p in prompts:
+            mine: List[TokenScore] = []
+            req = runner.open(("score", self._next_id))
+            self._next_id += 1
+            try:
+                for at in range(0, len(p) - 1, self.scheduler.ubatch):
+                    part = p[at:min(at + self.scheduler.ubatch, len(p) - 1)]            # (the last token's own logits are nobody's)
+                    given = p[at + 1:at + 1 + len(part)]
+                    logits = runner.step([(req, part, range(len(part)))])
+                    mine += PendingScores(logits, torch.tensor(given, dtype=torch.int32).to(logits.device), top, self.rt.status).scores(given)
+                self.rt.check_status()
+            finally:
+                runner.close(req)
+            out.append(mine)
+        return out
+
+    def greedy(self, prompt: Sequence[int], n_predict: int, stop: Optional[Sequence[int]] = None, draft=None):
+        """Greedy decode of one prompt: (new ids, timings {prefill, decode, n_decode, steps}), as
+        ``generate.greedy`` (``lua/lgml/generate.lua:19-34``).  With ``draft`` (a callable as in ``engine/drafts.py``: ids so far -> tokens, parents) every
+        step runs the last token and what may follow it as a tree, and takes what the model would have chosen: up to as many tokens as the tree
+        is deep, and one.  The ids are those of the argmax either way; where two logits are all but equal, the rounding of a step with another number of
+        tokens can decide."""
         runner = self.runner
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise ValueError("greedy: empty prompt")
         if n_predict <= 0:
-            return [], {"prefill": 0.0, "decode": 0.0, "n_decode": 0}
+            return [], {"prefill": 0.0, "decode": 0.0, "n_decode": 0, "steps": 0}
         req = runner.open(("greedy", self._next_id))
         self._next_id += 1
         out: List[int] = []
@@ -335,12 +402,40 @@ class Engine:
             cur = int(ops.argmax_rows(logits, tok).item())
             t1 = time.perf_counter()
             out.append(cur)
+            steps = 0
+            chain = [cur]           # ids that are not in the cache yet; the last of them the latest
             while len(out) < n_predict and cur not in stop:
-                logits = runner.step([(req, [cur], [0])])
-                cur = int(ops.argmax_rows(logits, tok).item())
-                out.append(cur)
+                steps += 1
+                if draft is None:
+                    logits = runner.step([(req, [cur], [0])])
+                    cur = int(ops.argmax_rows(logits, tok).item())
+                    out.append(cur)
+                    continue
+                drafted, parents = draft(prompt + out)
+                room = min(ops.TREE_TOKENS, self.scheduler.max_position - req.n_tokens) - len(chain)
+                drafted, parents = [int(t) for t in drafted][:max(room, 0)], [int(p) for p in parents][:max(room, 0)]
+                m = len(chain)
+                tokens = chain + drafted
+                logits = runner.step_tree([(req, tokens, list(range(-1, m - 1)) + [m - 1 if p < 0 else m + p for p in parents])])
+                best = ops.argmax_rows(logits, torch.empty(len(tokens), dtype=torch.int32, device=self.rt.device)).tolist()
+                at, taken = m - 1, []
+                while True:
+                    cur = best[at]
+                    out.append(cur)
+                    if len(out) >= n_predict or cur in stop:
+                        break
+                    at = next((m + i for i, (t, p) in enumerate(zip(drafted, parents)) if t == cur and (m - 1 if p < 0 else m + p) == at), -1)
+                    if at < 0:
+                        break
+                    taken.append(at)
+                # cells that lie as a chain would stay; the tokens behind them are run again at the head of the next step
+                whole = 0
+                while whole < len(taken) and taken[whole] == m + whole:
+                    whole += 1
+                runner.keep(req, m + whole)
+                chain = [tokens[i] for i in taken[whole:]] + [cur]
             t2 = time.perf_counter()
             self.rt.check_status()
         finally:
             runner.close(req)
-        return out, {"prefill": t1 - t0, "decode": t2 - t1, "n_decode": len(out) - 1}
+        return out, {"prefill": t1 - t0, "decode": t2 - t1, "n_decode": len(out) - 1, "steps": steps}

@@ -42,6 +42,7 @@ class DecodeBatch:
         self.min_kv_len = reach // 2 + 1 if reach and even else 1       # ... and the shortest
         self.decode_splits = None
         self.shared = {}                # what one layer of the step keeps for later layers (by name)
+        self.cells = self.visible = None        # (a token's key lies at its position)
         total = 3 * S + (S + 1) + 4 * S + S * sum(self.widths)
         self.total = total
         self.dev = torch.zeros(total, dtype=torch.int32, device=device)

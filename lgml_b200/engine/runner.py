@@ -17,6 +17,7 @@ import torch
 
 from .. import host, ops
 from ..cache import CacheManager, PoolFull, Request
+from ..cache.manager import EIGHT_BIT
 from ..models import build_model
 from ..weights import load_tensors, random_tensors
 from .batch import StepBatch
@@ -74,11 +75,19 @@ class StepError(ValueError):
 
 class ModelRunner:
     def __init__(self, model, rt: Runtime, n_pages: int, max_slots: int = 4, max_step_tokens: int = 0, use_graphs: bool = True,
-                 prefix_cache: bool = False):
+                 prefix_cache: bool = False, cache_dtype: Optional[torch.dtype] = None):
+        """``cache_dtype``: the type of keys and values in the pages (None: the compute type; ``torch.float8_e4m3fn``: eight bits, for models of plain
+        attention in bfloat16)."""
         self.model = model
         self.rt = rt
+        if cache_dtype not in (None, rt.dtype):
+            if cache_dtype != EIGHT_BIT:
+                raise ValueError(f"the cache holds {rt.dtype} or {EIGHT_BIT}, not {cache_dtype}")
+            if rt.dtype != torch.bfloat16 or not model.takes_trees:
+                raise ValueError("a cache of eight bits is for models of plain attention layers (head sizes in steps of 16 up to 128) that run in bfloat16")
         self.cache = CacheManager(model.cache_layout(), n_pages=n_pages, max_slots=max_slots, dtype=rt.dtype,
-                                  device=rt.device, max_step_tokens=max_step_tokens, prefix_cache=prefix_cache)
+                                  device=rt.device, max_step_tokens=max_step_tokens, prefix_cache=prefix_cache, page_dtype=cache_dtype)
+        self._drafted = {}              # requests of the last ``step_tree`` -> the cells it wrote for them
         # a ring of pinned staging buffers: a buffer is reused only after its copy has run
         self._pinned = [[torch.empty(1 << 16, dtype=torch.int32).pin_memory(), None] for _ in range(4)]
         self.steps = 0
@@ -238,6 +247,8 @@ class ModelRunner:
         if self.cache.state_groups or any(g.spec.window is not None for g in self.cache.groups):
             return False
         padded = prompt_graph_length(n, page)
+        if self.cache.page_dtype == EIGHT_BIT and padded > ops.TREE_TOKENS:
+            return False            # (its pages are read back into memory whose size follows the context)
         limit = self.model.max_position or (self.cache.n_pages * page)
         return req.n_tokens + padded <= min(limit, self._graph_widths[0] * page if self._graph_widths else limit)
 
@@ -301,6 +312,48 @@ class ModelRunner:
         if not want_rows:
             return logits[:0]
         return logits[torch.tensor(want_rows, dtype=torch.long, device=logits.device)]
+
+    # ---- drafted tokens ----------------------------------------------------------------
+    def step_tree(self, entries: Sequence[Tuple[Request, Sequence[int], Sequence[int]]]) -> torch.Tensor:
+        """entries: (request, tokens, parents): up to 64 tokens a request that form a tree, ``parents[i]`` the place of the token that token i
+        follows (before i; -1: the request's tokens so far).  Runs them all in one step and returns the float32 logits of every token
+        [tokens, vocab].  Nothing is committed: ``keep`` says how many of a request's tokens, from its first on, stay in the cache; what a
+        step does not keep is written over by the next."""
+        if self.rt.dtype != torch.bfloat16 or not self.model.takes_trees:
+            raise StepError("drafted tokens are for models of plain attention layers that run in bfloat16")
+        for req, tokens, parents in entries:
+            if len(parents) != len(tokens):
+                raise StepError(f"request {req.id!r}: {len(tokens)} tokens and {len(parents)} parents")
+            if len(tokens) > ops.TREE_TOKENS:
+                raise StepError(f"request {req.id!r} brings {len(tokens)} drafted tokens, a step takes {ops.TREE_TOKENS}")
+            for i, p in enumerate(parents):
+                if not -1 <= int(p) < i:
+                    raise StepError(f"request {req.id!r}: token {i} follows token {p}, which is not before it")
+        whole = [(req, tokens, range(len(tokens))) for req, tokens, _ in entries]
+        brought = self.validate(whole)
+        self._reserve_all([(req, len(tokens)) for req, tokens, _ in entries])
+        stage = self._pinned[self.steps % len(self._pinned)]
+        if stage[1] is not None:
+            stage[1].synchronize()
+        batch = StepBatch(self.cache, [e[0] for e in entries], brought, [e[2] for e in whole], self.rt.device, stage[0])
+        self._mark_busy(stage)
+        batch.tree([[int(p) for p in e[2]] for e in entries])
+        self.last_batch = batch
+        logits = self.model.forward(self.rt, batch)
+        self._drafted = {e[0]: (e[0].n_tokens, list(e[2])) for e in entries}
+        self.steps += 1
+        self.tokens_run += sum(len(e[1]) for e in entries)
+        return logits
+
+    def keep(self, req: Request, n: int) -> None:
+        """The first ``n`` tokens that the last ``step_tree`` ran for the request stay in its cache: each must follow the one before it."""
+        at, parents = self._drafted.get(req, (None, ()))
+        if at is None or at != req.n_tokens or req.closed:
+            raise StepError(f"request {req.id!r} has no drafted tokens to keep")
+        if not 0 <= n <= len(parents) or any(int(parents[i]) != i - 1 for i in range(n)):
+            raise StepError(f"request {req.id!r}: its first {n} drafted tokens are no chain")
+        del self._drafted[req]
+        self.cache.commit(req, n)
 
     def decode_step(self, requests: Sequence[Request], device_tokens: torch.Tensor) -> torch.Tensor:
         """One decode step whose token ids are already on the device (int32, one per request),

@@ -49,6 +49,7 @@ class GenRequest:
     admitted_at: int = -1
     preemptions: int = 0
     repeat_run: int = 0
+    scores: Optional[list] = None     # of every generated token, when asked for: ``TokenScore`` (``engine/scores.py``)
 
     tokens: List[int] = field(default_factory=list)   # prompt + generated, kept as one list
 

@@ -20,6 +20,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..cache import PagedKV
 from ..parts.norm import PendingDelta, ScaledTerms, UnitMix
 from ..parts.streams import PendingStreams
 from ..weights import VECTOR, TensorSpec
@@ -121,6 +122,12 @@ class DecoderModel:
             self.pass_rows = tensors[self.pass_rows_name].float().contiguous()
 
     # ---- cache -------------------------------------------------------------------------
+    @property
+    def takes_trees(self) -> bool:
+        """Whether every layer is plain attention over its own pages, without state of its own: what a cache of eight bits and steps of drafted
+        tokens need (``Attention.takes_trees``)."""
+        return all(isinstance(b.cache_spec(), PagedKV) and getattr(getattr(b, "mixer", None), "takes_trees", False) for b in self.blocks)
+
     def cache_layout(self) -> Dict[int, object]:
         """schedule index -> the cache spec of the calls that own a cache."""
         out = {}

@@ -3137,6 +3137,31 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     return out
 
 
+def cached_attention(q, batch, cache, out, n_heads: int, scale: float, window: int, status: torch.Tensor) -> torch.Tensor:
+    """Attention of a step over a cache of eight bits, or of a step whose tokens form trees: requests that bring up to 64 tokens by ``tree_attention``;
+    of longer portions the pages are read back as bfloat16 (``kv_read``) for the prompt kernels, whose products a tile of many rows shares."""
+    visible = getattr(batch, "visible", None)
+    table, k, v = cache.block_table, cache.k, cache.v
+    short = [n for n in batch.seq_lens if n <= TREE_TOKENS]
+    if short:
+        tree_attention(q, batch.positions, batch.seq_start, batch.seq_pos0, table, k, v, out, n_heads, scale, window, status, max_new_tokens=max(short),
+                       max_kv_len=batch.max_kv_len, k_exps=cache.k_exps, v_exps=cache.v_exps, visible=visible)
+    if len(short) == len(batch.seq_lens):
+        return out
+    if visible is not None:
+        raise KernelError(f"cached_attention: a tree has at most {TREE_TOKENS} tokens, a request brings {batch.max_q_len}")
+    d, hkv = k.shape[3], k.shape[1]
+    pages, table = batch.read_back(cache.group, TREE_TOKENS)
+    k, v = kv_read(k, v, cache.k_exps, cache.v_exps, pages, status)
+    fast = prefill_tc_supports(q, out)
+    if d in (64, 128) and fast:
+        tiles = batch.attention_tiles(prefill_twin_tile_tokens(n_heads, hkv), TREE_TOKENS, remember=False)
+        n_ranges = prefill_twin_ranges(batch, tiles, prefill_twin_ctas(n_heads, hkv), window)
+        return prefill_attention_twin(q, batch.positions, tiles, table, k, v, out, n_heads, scale, window, status, n_ranges=n_ranges)
+    tile, attend = (prefill_tc_tile_tokens, prefill_attention_tc) if fast else (prefill_tile_tokens, prefill_attention)
+    return attend(q, batch.positions, batch.attention_tiles(tile(n_heads, hkv), TREE_TOKENS, remember=False), table, k, v, out, n_heads, scale, window, status)
+
+
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs ranks entropies top_ids top_logprobs")
 
 

@@ -55,6 +55,11 @@ class Attention(Part):
         captured is up to the parts it is given."""
         return all(getattr(p, "graph_safe", False) for p in (self.position, self.q_norm, self.k_norm) if p is not None)
 
+    @property
+    def takes_trees(self):
+        """Whether its cache may have eight bits and its tokens may form a tree: ``ops.rope_kv_store`` and ``ops.tree_attention`` do its work then."""
+        return isinstance(self.position, RotaryPosition) and not self.softcap and self.head_dim % 16 == 0 and self.head_dim <= ops.TREE_MAX_DIM
+
     def cache_spec(self):
         return PagedKV(self.n_kv_heads, self.head_dim, self.window)
 

@@ -59,8 +59,16 @@ def store_kv(rt, qkv, batch, cache, n_heads: int, n_kv_heads: int, head_dim: int
     the cache as they are and return q: what a position part that has already done its own
     work on q and k (or does none) finishes with."""
     none = torch.zeros(1, dtype=torch.float32, device=rt.device)
+    if cache.k_exps is not None or getattr(batch, "cells", None) is not None:
+        return _store(rt, qkv, batch, cache, none, 0, "half", n_heads, n_kv_heads, head_dim)
     return ops.rope_kv_write(qkv, batch.positions, batch.seq_of_token, cache.block_table, none, 0, "half", cache.k, cache.v,
                              n_heads, n_kv_heads, head_dim, rt.status, write_kv=cache.writable)
+
+
+def _store(rt, qkv, batch, cache, inv_freq, n_rot: int, pairing: str, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """The same into a cache of eight bits, or into cells that are not the tokens' positions (``StepBatch.tree``)."""
+    return ops.rope_kv_store(qkv, batch.positions, batch.seq_of_token, cache.block_table, inv_freq, n_rot, pairing, cache.k, cache.v, n_heads, n_kv_heads,
+                             head_dim, rt.status, cells=getattr(batch, "cells", None), k_exps=cache.k_exps, v_exps=cache.v_exps, write_kv=cache.writable)
 
 
 class RotaryPosition(Part):
@@ -82,6 +90,8 @@ class RotaryPosition(Part):
         ``ops.Partials`` of it.  Writes this step's k and v into ``cache`` (unless it belongs
         to another layer call: ``cache.writable``) and returns q [tokens, H D] in the cache's
         type, ready for attention."""
+        if cache.k_exps is not None or getattr(batch, "cells", None) is not None:
+            return _store(rt, qkv, batch, cache, self.inv_freq, self.n_rot, self.pairing, n_heads, n_kv_heads, head_dim)
         return ops.rope_kv_write(qkv, batch.positions, batch.seq_of_token, cache.block_table, self.inv_freq, self.n_rot,
                                  self.pairing, cache.k, cache.v, n_heads, n_kv_heads, head_dim, rt.status, write_kv=cache.writable)
 
