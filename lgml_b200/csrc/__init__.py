@@ -60,6 +60,7 @@ LIBRARIES: Dict[str, tuple] = {
     "rglru": ("rglru.cu", []),
     "kv_store": ("kv_store.cu", []),
     "attention_tree": ("attention_tree.cu", []),
+    "attention_tree_tall": ("attention_tree_tall.cu", []),
     "logprobs": ("logprobs.cu", []),
 }
 
@@ -153,6 +154,8 @@ LIBRARY_HEADERS: Dict[str, List[str]] = {
     "rglru": ["few_rows.cuh"],
     "gemm_f32": ["bf16_thirds.cuh"],
     "ssd": ["bf16_thirds.cuh"],
+    "attention_tree": ["tree_common.cuh"],
+    "attention_tree_tall": ["tree_common.cuh"],
 }
 
 

@@ -27,23 +27,14 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include "common.cuh"
+#include "tree_common.cuh"
 
 LGML_DEFINE_LAST_ERROR(lgml_attention_tree)
 
 namespace {
-constexpr int PAGE = 64;
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int MAX_NEW = 64;             // bits of a mask
-constexpr int MAX_SPLITS = 256, MAX_CLUSTER = 8;
 
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
-__device__ __forceinline__ unsigned half2_of_codes(unsigned short two) {
-    unsigned r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
-    return r;
-}
 __device__ __forceinline__ unsigned transpose8(unsigned a) {
     unsigned r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -57,33 +48,6 @@ __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, uns
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy_16(uint32_t dst, const void *src, bool there) {
-    const int bytes = there ? 16 : 0;            // 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ unsigned block_of_cluster() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory"); }
-// What block `rank` of the cluster has where this block has p.
-__device__ __forceinline__ float2 load_there(const float *p, int rank) {
-    uint32_t at;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
-    return v;
 }
 
 // N 32-bit words of shared memory, at most four at a time.
@@ -117,13 +81,6 @@ template <int KS, bool Q8> struct Cut {
     static __device__ __forceinline__ int key_entry(int ks, int c) { return (ks / (KE / 4)) * 4 * KE + c * KE + (ks % (KE / 4)) * 4; }
     static __device__ __forceinline__ int value_entry(int mt, int g) { return (mt / (VE / 2)) * 8 * VE + g * VE + (mt % (VE / 2)) * 2; }
 };
-
-// What a part with maximum m counts for beside others up to M (nothing seen: 0, or NaN, which stays one).
-__device__ __forceinline__ float share_of(float m, float M) { return m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M); }
-__device__ __forceinline__ void store_row(__nv_bfloat16 *dst, float2 o, float l) {
-    const float inv = 1.f / l;
-    *reinterpret_cast<__nv_bfloat162 *>(dst) = l == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o.x * inv, o.y * inv);
-}
 
 template <int KS, int NT, bool Q8>
 __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
@@ -476,14 +433,13 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
             l += p[D + 1] * f;
             o.x += p[d] * f, o.y += p[d + 1] * f;
         }
-        const size_t tok = row0 + (r0 + row) / group, head = kvh * group + (r0 + row) % group;
         if (n_splits == 1) {
-            store_row(out + tok * ldo + head * D + d, o, l);
+            store_row(row_at(out, ldo, row0, r0 + row, group, kvh, D, d), o, l);
         } else if (clustered) {
             *reinterpret_cast<float2 *>(merge + (size_t)row * (D + 2) + d) = o;         // (no other thread reads it here)
             if (d == 0) fin[row][0] = M, fin[row][1] = l;
         } else {
-            const size_t at = (tok * H + head) * n_splits + split;
+            const size_t at = ((size_t)(row0 + (r0 + row) / group) * H + kvh * group + (r0 + row) % group) * n_splits + split;
             *reinterpret_cast<float2 *>(part_o + at * D + d) = o;
             if (d == 0) part_ml[at] = make_float2(M, l);
         }
@@ -492,83 +448,9 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     // ---- the cluster's ranges together: each block joins a share of the results ----
     __syncwarp();
     cluster_sync();
-    for (int i = (int)block_of_cluster() * THREADS + tid; i < ROWS * (D / 2); i += n_splits * THREADS) {
-        const int row = i / (D / 2), d = 2 * (i - row * (D / 2));
-        if (r0 + row >= n_rows) break;
-        float2 ml[MAX_CLUSTER], part[MAX_CLUSTER];
-#pragma unroll
-        for (int j = 0; j < MAX_CLUSTER; ++j)
-            if (j < n_splits) ml[j] = load_there(fin[row], j), part[j] = load_there(merge + (size_t)row * (D + 2) + d, j);
-        float M = -INFINITY, l = 0.f;
-        float2 o = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < MAX_CLUSTER; ++j)
-            if (j < n_splits) M = fmaxf(M, ml[j].x);
-#pragma unroll
-        for (int j = 0; j < MAX_CLUSTER; ++j)
-            if (j < n_splits) {
-                const float f = share_of(ml[j].x, M);
-                l += ml[j].y * f;
-                o.x += part[j].x * f, o.y += part[j].y * f;
-            }
-        store_row(out + (size_t)(row0 + (r0 + row) / group) * ldo + (size_t)(kvh * group + (r0 + row) % group) * D + d, o, l);
-    }
+    join_cluster<ROWS, D, THREADS>(merge, fin, n_splits, n_rows - r0, [&](int row, int d) { return row_at(out, ldo, row0, r0 + row, group, kvh, D, d); });
     __syncwarp();
     cluster_sync();                         // (the others' shared memory is read until here)
-}
-
-// The ranges of one (token, head) in their order: a warp each.
-constexpr int JOIN_WARPS = 2;
-__global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml,
-                                                                    const int *__restrict__ seq_start, int limit, int n_tokens, __nv_bfloat16 *__restrict__ out,
-                                                                    int ldo, int n_splits, int H, int D) {
-    pdl_trigger();
-    pdl_wait();
-    const int s = blockIdx.x / limit, j = blockIdx.x - s * limit, lane = threadIdx.x & 31;
-    const int head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
-    const int row0 = act_load(seq_start + s), n = act_load(seq_start + s + 1) - row0;
-    if (j >= n || n > limit || head >= H || row0 < 0 || row0 + n > n_tokens) return;
-    const size_t at = ((size_t)(row0 + j) * H + head) * n_splits;
-    // lane i has the maxima and sums of ranges i, i + 32, ..; eight ranges' outputs are under way at a time
-    constexpr int PER_LANE = MAX_SPLITS / 32;
-    float2 ml[PER_LANE];
-    float M = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int p = 0; p < PER_LANE; ++p) {
-        ml[p] = lane + 32 * p < n_splits ? act_load(part_ml + at + lane + 32 * p) : make_float2(-INFINITY, 0.f);
-        M = fmaxf(M, ml[p].x);
-    }
-    M = warp_max(M);
-#pragma unroll
-    for (int p = 0; p < PER_LANE; ++p) {
-        ml[p].x = share_of(ml[p].x, M);
-        l += ml[p].y * ml[p].x;
-    }
-    l = warp_sum(l);
-    float2 o[2] = {};
-#pragma unroll
-    for (int p = 0; p < PER_LANE; ++p)
-        for (int i0 = 32 * p; i0 < min(n_splits, 32 * p + 32); i0 += 8) {
-            float2 v[8][2];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int d = 2 * (lane + 32 * u);
-                    v[e][u] = i0 + e < n_splits && d < D ? act_load(reinterpret_cast<const float2 *>(part_o + (at + i0 + e) * D + d)) : make_float2(0.f, 0.f);
-                }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float f = __shfl_sync(0xffffffffu, ml[p].x, (i0 + e) & 31);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) o[u].x += v[e][u].x * f, o[u].y += v[e][u].y * f;
-            }
-        }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int d = 2 * (lane + 32 * u);
-        if (d < D) store_row(out + (size_t)(row0 + j) * ldo + (size_t)head * D + d, o[u], l);
-    }
 }
 
 template <int KS, int NT, bool Q8, typename... Args>
@@ -637,7 +519,5 @@ LGML_API int lgml_tree_attention(const void *q, int ldq, const int *positions, c
     int rc = k_exps ? launch_dim<true>(LGML_ARGS) : launch_dim<false>(LGML_ARGS);
 #undef LGML_ARGS
     if (rc || n_splits <= MAX_CLUSTER) return rc;
-    lgml_launch(tree_join_kernel, dim3(n_seqs * limit, (H + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, part_o, part_ml, seq_start, limit,
-                n_tokens, (__nv_bfloat16 *)out, ldo, n_splits, H, D);
-    return lgml_launch_status("tree_attention_join");
+    return tree_join(part_o, part_ml, seq_start, n_seqs, limit, n_tokens, out, ldo, n_splits, H, D, stream);
 }

@@ -2932,6 +2932,7 @@ def paged_attention(q, batch, cache, out, n_heads: int, scale: float, window: in
 E4M3 = torch.float8_e4m3fn
 TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
 TREE_MAX_DIM = 128
+TREE_TALL_ROWS = 33         # rows of a KV head (tokens x heads) from which it takes 128 of them a block, on tcgen05
 TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
 
@@ -3080,11 +3081,12 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     return k_out, v_out
 
 
-def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64) -> int:
+def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64, tall: bool = False) -> int:
     """Into how many ranges of pages ``tree_attention`` cuts a request's cells."""
-    blocks = max(n_seqs * n_kv_heads * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32)), 1)
+    height, per_sm = (128, 2) if tall else (8 if rows <= 8 else 16 if rows <= 16 else 32, 4)
+    blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
-    return max(1, min(-(-pages // 2), (4 * sm_count()) // blocks, 64))
+    return max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
 
 
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
@@ -3118,8 +3120,10 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         _are(who, dev, torch.int64, 1, "masks", visible)
         if visible.numel() != n:
             raise KernelError(f"{who}: one mask a token")
+    rows = max_new_tokens * (n_heads // hkv)
+    tall = rows >= TREE_TALL_ROWS and d in (64, 128) and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
     if n_splits is None:
-        n_splits = tree_splits(seqs, hkv, max_new_tokens * (n_heads // hkv), max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page))
+        n_splits = tree_splits(seqs, hkv, rows, max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page), page, tall)
     if n_splits > TREE_CLUSTER:
         need = n * n_heads * n_splits * (d + 2)
         if scratch is None:
@@ -3127,13 +3131,13 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         _are(who, dev, torch.float32, 1, "scratch", scratch)
         if scratch.numel() < need:
             raise KernelError(f"{who}: scratch of {scratch.numel()} floats, {need} needed")
-    fn = _fn("attention_tree", "lgml_tree_attention", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                                       c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                                                       c_void_p, c_void_p])
-    _check("attention_tree", fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
-                                blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
-                                scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
-                                status.data_ptr(), _stream()), who)
+    lib, name = ("attention_tree_tall", "lgml_tree_attention_tall") if tall else ("attention_tree", "lgml_tree_attention")
+    fn = _fn(lib, name, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                         c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+    _check(lib, fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
+                   blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
+                   scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
+                   status.data_ptr(), _stream()), who)
     return out
 
 
