@@ -1,13 +1,18 @@
 // Attention of the new tokens of a request over its paged cache (attention_tree.cu has the definition) where a KV head has many rows: tokens x heads
 // of 33 and more.  There the products are what takes time, so they are on tcgen05, 128 rows a block:
 //     S[128, 64] = Q[128, D] . K_page^T        O[128, D] += P[128, 64] . V_page        accumulators in tensor memory
-// Warps 0-3 do the softmax, a thread a row; warps 4-7 bring the pages, the first thread of warp 4 issues the products, the scores of the next page ahead of
-// this page's P V.  Operands lie in shared memory in rows of 128 bytes, swizzled; V is the N-major operand.  The running output is
-// corrected only when a row's maximum has grown by more than 2^8 since its sums' (it stays in tensor memory all along).
+// Warps 0-3 do the softmax, a thread a row, and write P back into tensor memory, over the scores it came from; warps 4-6 bring the pages, into two stages
+// of keys and of values; the first thread of warp 7 issues the products.  There are two buffers of scores: those of page it + 2 are issued behind the P V
+// product of page it, which read the buffer they go to, so a page's scores are there before the softmax of the page ahead of it is done, and the
+// only chain is softmax after softmax.  (Products of one thread complete in the order of issue.)  Operands lie in shared memory in rows of 128 bytes,
+// swizzled; V is the N-major operand.  The running output stays in tensor memory; the softmax threads correct it only when a row's maximum
+// has grown by more than 2^8 since its sums'.
+// Every mbarrier is of one parity of pages, and what its next phase needs comes after its waiters have seen this one, so none is missed.
+// Tensor memory is taken behind the wait for the kernels ahead, so it is never held against one of them, and the kernels behind start when this one is done.
 //
 // Pages of e4m3 become float16 on the way to shared memory, exactly: 16 codes a load, converted by the threads that load them while the
 // softmax of the page before runs.  Their powers of two stay outside: a key's multiplies its column of scores, a value's joins its column's
-// exponent, and q is scaled row by row, as in attention_tree.cu.  Pages in bfloat16 are copied as they are.
+// exponent, and q is scaled row by row, as in attention_tree.cu.  Pages in bfloat16 are copied as they are, a page ahead.
 //
 // Every column that a row may not see is a bit of a 64-bit word, tested only in pages that some row does not see whole.  There, values that are
 // not finite become zeros before the product (0 x NaN), and are added at the end to the rows that see them.
@@ -19,8 +24,8 @@ LGML_DEFINE_LAST_ERROR(lgml_attention_tree_tall)
 namespace {
 constexpr int ROWS = 128;
 constexpr int THREADS = 256;
-constexpr int LOADERS = 128;                 // threads of warps 4-7
-constexpr int ISSUER = 128;
+constexpr int LOADERS = 96;                  // threads of warps 4-6
+constexpr int ISSUER = 224;                  // the first thread of warp 7
 constexpr uint32_t SPIN_LIMIT = 1u << 20;    // polls of up to WAIT_HINT_NS each: about a second
 constexpr uint32_t WAIT_HINT_NS = 1000;
 constexpr int STATUS_TIMEOUT = 14;
@@ -31,6 +36,9 @@ constexpr float RESCALE_STEP = 8.f;
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
     uint4 v;
@@ -77,6 +85,14 @@ __device__ __forceinline__ void tcgen05_mma_f16(uint32_t tmem_d, uint64_t desc_a
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A in tensor memory: its row i in lane i, two 16-bit elements of K a 32-bit column
+__device__ __forceinline__ void tcgen05_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tcgen05_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -133,15 +149,15 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     constexpr int KB = D / 64;                        // 64-element blocks along the head
     constexpr uint32_t Q_BYTES = KB * ROWS * 128, K_BYTES = KB * PAGE * 128;
     constexpr int HALF = D / 2;
-    constexpr int SIZE = Q8 ? 1 : 2, LOADS = PAGE * D * SIZE / 16 / LOADERS, PER_ROW = D * SIZE / 16;        // 16-byte loads of a page's keys: a thread's, a row's
+    constexpr int SIZE = Q8 ? 1 : 2, PER_ROW = D * SIZE / 16, CHUNKS = PAGE * PER_ROW, LOADS = (CHUNKS + LOADERS - 1) / LOADERS;       // 16-byte loads of a page's keys: a row's, all, a thread's
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *Qs = base, *Ks = Qs + Q_BYTES, *Vs = Ks + 2 * K_BYTES, *Ps = Vs + K_BYTES;
-    __shared__ __align__(16) float2 col_s[2][PAGE];       // per column of a page: its scores' factor, what is added to them
-    __shared__ __align__(16) float vf_s[2][PAGE];         // and what its probability counts for in the sum
+    uint8_t *Qs = base, *Ks = Qs + Q_BYTES, *Vs = Ks + 2 * K_BYTES;         // two stages of keys, two of values
+    __shared__ __align__(16) float2 col_s[4][PAGE];       // per column of page it (it % 4): its scores' factor, what is added to them
+    __shared__ __align__(16) float vf_s[4][PAGE];         // and what its probability counts for in the sum
     __shared__ __align__(8) float fin[ROWS][2];
-    __shared__ float corr_s[ROWS], unscale_s[ROWS];
-    __shared__ uint64_t s_bar, o_bar;
+    __shared__ float unscale_s[ROWS];
+    __shared__ uint64_t k_full[2], v_full[2], s_full[2], p_full[2], o_done[2];        // by the page's parity
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s, odd_s, ok_s[4];               // ok_s[it % 4]: whether page it is there
     volatile int *abort_flag = &abort_s;
@@ -189,103 +205,23 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     const int pb = first_page + split * pps, n_it = max(min(pps, end_page - pb), 0);
 
     if (tid == 0) {
-        mbar_init(&s_bar, 1);
-        mbar_init(&o_bar, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], LOADERS);
+            mbar_init(&v_full[i], LOADERS);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], ROWS);
+            mbar_init(&o_done[i], 1);
+        }
         abort_s = odd_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tcgen05_alloc(&tmem_base_s, TMEM_COLS);
-    tcgen05_fence_before();
-    __syncthreads();
-    tcgen05_fence_after();
-    const uint32_t tmem_base = tmem_base_s, lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const float scale_log2 = scale * 1.4426950408889634f;
-    bool alive = true;
-
-    // ---- the pages: warps 4-7 ----
-    const int l = tid - LOADERS;
-    auto page_of = [&](int it) {
-        const int page = pb + it < max_blocks ? early_int(block_table + (size_t)s * max_blocks + pb + it) : -1;
-        return page >= 0 && page < n_pages ? page : -1;
-    };
-    // Load u of a thread: row (l + 128 u) / PER_ROW of the page, 16 bytes from chunk (l + 128 u) % PER_ROW on.
-    auto fetch = [&](uint4 (&raw)[LOADS], const uint8_t *pages, int it) {
-        const int page = page_of(it), left = n_cells - (pb + it) * PAGE;
-        const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u;
-            raw[u] = page >= 0 && at / PER_ROW < left ? __ldcg(reinterpret_cast<const uint4 *>(src) + at) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    // ... as float16 in shared memory; in a page that not every row sees whole (check), without what is not finite.
-    auto convert = [&](uint32_t dst, const uint4 (&raw)[LOADS], bool check) {
-        bool odd = false;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u, r = at / PER_ROW, ch = 2 * (at - r * PER_ROW);
-            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                h[j] = half2_of_codes((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
-                if (check) h[j] = finite_pair(h[j], 0x7c007c00u, odd);
-            }
-            const uint32_t block = dst + (ch >> 3) * (PAGE * 128);
-            st_shared_16(block + swz(r, ch & 7), h[0], h[1], h[2], h[3]);
-            st_shared_16(block + swz(r, (ch & 7) + 1), h[4], h[5], h[6], h[7]);
-        }
-        if (odd) odd_s = 1;
-    };
-    auto columns = [&](int it) {            // what the softmax of page it has to know of its columns
-        const int page = page_of(it);
-        if (l == 0) ok_s[it & 3] = page >= 0;
-        if (l == 0 && page < 0) atomicExch(status, 3);
-        if (Q8 && l < PAGE) {
-            const size_t vec = ((size_t)max(page, 0) * Hkv + kvh) * PAGE + l;
-            const bool there = page >= 0 && (pb + it) * PAGE + l < n_cells;
-            const int ke = there ? min((int)__ldcg(k_exps + vec), 246) - 127 : 0, ve = there ? min((int)__ldcg(v_exps + vec), 246) - 127 : 0;
-            col_s[it & 1][l] = make_float2(scale_log2 * power_of_two(ke), (float)ve);
-            vf_s[it & 1][l] = power_of_two(-ve);
-        }
-    };
-    // bfloat16: asynchronous copies
-    auto copy_page = [&](uint32_t dst, const uint8_t *pages, int it) {
-        const int page = page_of(it), left = n_cells - (pb + it) * PAGE;
-        const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D * 2;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
-            copy_16(dst + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7), src + (size_t)at * 16, page >= 0 && r < left);
-        }
-    };
-    const uint32_t ks0 = smem_u32(Ks), vs0 = smem_u32(Vs);
     pdl_wait();
-    if (warp >= 4) {
-        for (int it = 0; it < min(n_it, 2); ++it) {
-            columns(it);
-            if (Q8) {
-                uint4 raw[LOADS];
-                fetch(raw, k_pages, it);
-                convert(ks0 + it * K_BYTES, raw, false);
-            } else {
-                copy_page(ks0 + it * K_BYTES, k_pages, it);
-            }
-        }
-        if (n_it > 0) {
-            if (Q8) {
-                uint4 raw[LOADS];
-                fetch(raw, v_pages, 0);
-                convert(vs0, raw, !whole(pb));
-            } else {
-                copy_page(vs0, v_pages, 0);
-            }
-        }
-        copies_commit();
-    } else {
+    if (warp == 1) tcgen05_alloc(&tmem_base_s, TMEM_COLS);
+    {
         // queries: row r = (token, head) r0 + r; through L2, they were just written
         constexpr int CH = D / 8;
-        for (int c = tid; c < ROWS * CH; c += 128) {
+#pragma unroll
+        for (int c = tid; c < ROWS * CH; c += THREADS) {
             const int r = c / CH, ch = c - r * CH, rr = r0 + r;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (rr < n_rows) v = __ldcg(reinterpret_cast<const uint4 *>(q + (size_t)(row0 + rr / group) * ldq + (size_t)(kvh * group + rr % group) * D + ch * 8));
@@ -314,48 +250,210 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
             *reinterpret_cast<uint4 *>(Qs + (ch >> 3) * (ROWS * 128) + swz(r, ch & 7)) = v;
         }
     }
-    copies_wait<0>();
     fence_async_smem();
+    tcgen05_fence_before();
     __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = tmem_base_s, lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const float scale_log2 = scale * 1.4426950408889634f;
+    bool alive = true;
 
-    // ---- the products: one thread ----
-    constexpr uint32_t idesc_qk = make_idesc(ROWS, PAGE, 0, Q8 ? 0 : 1), idesc_pv = make_idesc(ROWS, D, 1, Q8 ? 0 : 1);
-    const uint64_t desc_q0 = make_desc(smem_u32(Qs), 16, 1024), desc_k0 = make_desc(ks0, 16, 1024);
-    const uint64_t desc_p0 = make_desc(smem_u32(Ps), 16, 1024), desc_v0 = make_desc(vs0, PAGE * 128, 1024);
-    auto issue_qk = [&](int it) {
-        const uint64_t dk = desc_k0 + (uint64_t)(((it & 1) * K_BYTES) >> 4);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const uint64_t da = desc_q0 + (uint64_t)(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4);
-            const uint64_t db = dk + (uint64_t)(((ks >> 2) * (PAGE * 128) + (ks & 3) * 32) >> 4);
-            tcgen05_mma_f16(tmem_base + ((it & 1) ? S1_COL : 0u), da, db, idesc_qk, ks > 0 ? 1u : 0u);
-        }
-        tcgen05_commit(&s_bar);
+    // ---- the pages: warps 4-6 ----
+    const int l = tid - ROWS;                // (of 96)
+    auto page_of = [&](int it) {
+        const int page = pb + it < max_blocks ? early_int(block_table + (size_t)s * max_blocks + pb + it) : -1;
+        return page >= 0 && page < n_pages ? page : -1;
     };
-    if (tid == ISSUER && n_it > 0) {
-        tcgen05_fence_after();
-        issue_qk(0);
-    }
-
+    // Load u of a thread: chunk l + 96 u of the page, 16 bytes of row chunk / PER_ROW.
+    auto fetch = [&](uint4 (&raw)[LOADS], const uint8_t *pages, int it, int page) {
+        const int left = n_cells - (pb + it) * PAGE;
+        const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int at = l + LOADERS * u;
+            raw[u] = page >= 0 && at < CHUNKS && at / PER_ROW < left ? __ldcg(reinterpret_cast<const uint4 *>(src) + at) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    // ... as float16 in shared memory; in a page that not every row sees whole (check), without what is not finite.
+    auto convert = [&](uint32_t dst, const uint4 (&raw)[LOADS], bool check) {
+        bool odd = false;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int at = l + LOADERS * u, r = at / PER_ROW, ch = 2 * (at - r * PER_ROW);
+            if (at >= CHUNKS) break;
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[j] = half2_of_codes((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                if (check) h[j] = finite_pair(h[j], 0x7c007c00u, odd);
+            }
+            const uint32_t block = dst + (ch >> 3) * (PAGE * 128);
+            st_shared_16(block + swz(r, ch & 7), h[0], h[1], h[2], h[3]);
+            st_shared_16(block + swz(r, (ch & 7) + 1), h[4], h[5], h[6], h[7]);
+        }
+        if (odd) odd_s = 1;
+    };
+    // What the softmax of page it has to know of its columns: the exponents of column l, as bytes ...
+    auto exponents = [&](int it, int page) -> int2 {
+        if (!Q8 || l >= PAGE || page < 0 || (pb + it) * PAGE + l >= n_cells) return make_int2(127, 127);
+        const size_t vec = ((size_t)page * Hkv + kvh) * PAGE + l;
+        return make_int2((int)__ldcg(k_exps + vec), (int)__ldcg(v_exps + vec));
+    };
+    // ... and what it makes of them.
+    auto columns = [&](int it, int page, int2 e) {
+        if (l == 0) ok_s[it & 3] = page >= 0;
+        if (l == 0 && page < 0) atomicExch(status, 3);
+        if (Q8 && l < PAGE) {
+            const int ke = min(e.x, 246) - 127, ve = min(e.y, 246) - 127;
+            col_s[it & 3][l] = make_float2(scale_log2 * power_of_two(ke), (float)ve);
+            vf_s[it & 3][l] = power_of_two(-ve);
+        }
+    };
+    // bfloat16: asynchronous copies
+    auto copy_page = [&](uint32_t dst, const uint8_t *pages, int it, int page) {
+        const int left = n_cells - (pb + it) * PAGE;
+        const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D * 2;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
+            if (at < CHUNKS) copy_16(dst + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7), src + (size_t)at * 16, page >= 0 && r < left);
+        }
+    };
+    const uint32_t ks0 = smem_u32(Ks), vs0 = smem_u32(Vs);
     float m_ref = -INFINITY, l_run = 0.f;
-    const float unscale = Q8 ? unscale_s[row] : 1.f;
-    for (int it = 0; it < n_it; ++it) {
-        const int pg = pb + it;
-        int need = 0;
-        uint4 raw_k[Q8 ? LOADS : 1], raw_v[Q8 ? LOADS : 1];
-        if (warp < 4) {
-            // ---- softmax ----
-            if (alive && !mbar_wait(&s_bar, it & 1, abort_flag, status)) alive = false;
+    if (warp >= 4 && warp < 7) {
+        // page it's stage is free when the products of page it - 2 have read it
+        auto wait_for = [&](uint64_t *bar, int it) {
+            if (it >= 2 && alive && !mbar_wait(&bar[it & 1], ((it - 2) >> 1) & 1, abort_flag, status)) alive = false;
+        };
+        // (page numbers come two pages ahead, codes and exponents one: each is a trip to L2 or beyond)
+        int page = n_it > 0 ? page_of(0) : -1, page1 = n_it > 1 ? page_of(1) : -1;
+        if (Q8) {
+            uint4 raw_k[LOADS], raw_v[LOADS];
+            int2 exps = make_int2(127, 127);
+            if (n_it > 0) {
+                exps = exponents(0, page);
+                fetch(raw_k, k_pages, 0, page);
+                fetch(raw_v, v_pages, 0, page);
+            }
+            for (int it = 0; it < n_it && alive; ++it) {
+                const int page2 = it + 2 < n_it ? page_of(it + 2) : -1;
+                wait_for(s_full, it);
+                columns(it, page, exps);
+                convert(ks0 + (it & 1) * K_BYTES, raw_k, false);
+                fence_async_smem();
+                mbar_arrive(&k_full[it & 1]);
+                if (it + 1 < n_it) {
+                    exps = exponents(it + 1, page1);
+                    fetch(raw_k, k_pages, it + 1, page1);
+                }
+                wait_for(o_done, it);
+                convert(vs0 + (it & 1) * K_BYTES, raw_v, !whole(pb + it));
+                fence_async_smem();
+                mbar_arrive(&v_full[it & 1]);
+                if (it + 1 < n_it) fetch(raw_v, v_pages, it + 1, page1);
+                page = page1, page1 = page2;
+            }
+        } else {
+            // (a page's keys are asked for, then the page before is handed on, then this one's values are asked for: they wait for the product of
+            //  two pages before, which waits for that page)
+            for (int it = 0; it <= n_it && alive; ++it) {
+                const int page2 = it + 2 < n_it ? page_of(it + 2) : -1;
+                if (it < n_it) {
+                    wait_for(s_full, it);
+                    columns(it, page, make_int2(127, 127));
+                    copy_page(ks0 + (it & 1) * K_BYTES, k_pages, it, page);
+                }
+                copies_commit();
+                auto values = [&]() {
+                    if (it < n_it) {
+                        wait_for(o_done, it);
+                        copy_page(vs0 + (it & 1) * K_BYTES, v_pages, it, page);
+                    }
+                    copies_commit();
+                    page = page1, page1 = page2;
+                };
+                if (it == 0) {
+                    values();
+                    continue;
+                }
+                copies_wait<1>();               // all but the keys just asked for
+                const int pr = it - 1;
+                fence_async_smem();
+                mbar_arrive(&k_full[pr & 1]);
+                if (!whole(pb + pr)) {
+                    bool odd = false;
+#pragma unroll
+                    for (int u = 0; u < LOADS; ++u) {
+                        const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
+                        if (at >= CHUNKS) break;
+                        const uint32_t where = vs0 + (pr & 1) * K_BYTES + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7);
+                        const uint4 v = ld_shared_16(where);
+                        st_shared_16(where, finite_pair(v.x, 0x7f807f80u, odd), finite_pair(v.y, 0x7f807f80u, odd), finite_pair(v.z, 0x7f807f80u, odd),
+                                     finite_pair(v.w, 0x7f807f80u, odd));
+                    }
+                    if (odd) odd_s = 1;
+                    fence_async_smem();
+                }
+                mbar_arrive(&v_full[pr & 1]);
+                values();
+            }
+        }
+    } else if (tid == ISSUER) {
+        // ---- the products ----
+        constexpr uint32_t idesc_qk = make_idesc(ROWS, PAGE, 0, Q8 ? 0 : 1), idesc_pv = make_idesc(ROWS, D, 1, Q8 ? 0 : 1);
+        const uint64_t desc_q0 = make_desc(smem_u32(Qs), 16, 1024), desc_k0 = make_desc(ks0, 16, 1024), desc_v0 = make_desc(vs0, PAGE * 128, 1024);
+        auto issue_scores = [&](int it) {
+            const uint64_t dk = desc_k0 + (uint64_t)(((it & 1) * K_BYTES) >> 4);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                const uint64_t da = desc_q0 + (uint64_t)(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4);
+                const uint64_t db = dk + (uint64_t)(((ks >> 2) * (PAGE * 128) + (ks & 3) * 32) >> 4);
+                tcgen05_mma_f16(tmem_base + (uint32_t)(it & 1) * S1_COL, da, db, idesc_qk, ks > 0 ? 1u : 0u);
+            }
+            tcgen05_commit(&s_full[it & 1]);
+        };
+        for (int it = 0; it < n_it && it < 2 && alive; ++it) {
+            alive = mbar_wait(&k_full[it], 0, abort_flag, status);
+            tcgen05_fence_after();
+            if (alive) issue_scores(it);
+        }
+        for (int it = 0; it < n_it && alive; ++it) {
+            const uint32_t ph = (it >> 1) & 1;
+            alive = mbar_wait(&p_full[it & 1], ph, abort_flag, status) && mbar_wait(&v_full[it & 1], ph, abort_flag, status);
+            tcgen05_fence_after();
+            if (!alive) break;
+            const uint64_t dv = desc_v0 + (uint64_t)(((it & 1) * K_BYTES) >> 4);
+#pragma unroll
+            for (int k2 = 0; k2 < PAGE / 16; ++k2)
+                tcgen05_mma_f16_ts(tmem_base + O_COL, tmem_base + (uint32_t)(it & 1) * S1_COL + (uint32_t)k2 * 8u, dv + (uint64_t)((k2 * 2048) >> 4), idesc_pv,
+                                   (it > 0 || k2 > 0) ? 1u : 0u);
+            tcgen05_commit(&o_done[it & 1]);
+            if (it + 2 < n_it) {
+                alive = mbar_wait(&k_full[it & 1], ((it + 2) >> 1) & 1, abort_flag, status);
+                tcgen05_fence_after();
+                if (alive) issue_scores(it + 2);
+            }
+        }
+    } else if (warp < 4) {
+        // ---- softmax ----
+        const float unscale = Q8 ? unscale_s[row] : 1.f;
+        for (int it = 0; it < n_it; ++it) {
+            const int pg = pb + it;
+            const uint32_t s_addr = lane_addr + (uint32_t)(it & 1) * S1_COL;
+            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[it & 1], (it >> 1) & 1, abort_flag, status));         // (a warp goes on, or stops, as one)
+            if (!alive) break;
             tcgen05_fence_after();
             const bool edge = !whole(pg) || !ok_s[it & 3];
             uint32_t r[PAGE];
 #pragma unroll
-            for (int c0 = 0; c0 < PAGE; c0 += 16) tcgen05_ld_16(lane_addr + ((it & 1) ? S1_COL : 0u) + (uint32_t)c0, *reinterpret_cast<uint32_t(*)[16]>(&r[c0]));
+            for (int c0 = 0; c0 < PAGE; c0 += 16) tcgen05_ld_16(s_addr + (uint32_t)c0, *reinterpret_cast<uint32_t(*)[16]>(&r[c0]));
             tcgen05_wait_ld();
             if (Q8) {
 #pragma unroll
                 for (int c = 0; c < PAGE; c += 2) {
-                    const float4 f = *reinterpret_cast<const float4 *>(&col_s[it & 1][c]);
+                    const float4 f = *reinterpret_cast<const float4 *>(&col_s[it & 3][c]);
                     r[c] = __float_as_uint(fmaf(__uint_as_float(r[c]) * unscale, f.x, f.y));
                     r[c + 1] = __float_as_uint(fmaf(__uint_as_float(r[c + 1]) * unscale, f.z, f.w));
                 }
@@ -381,108 +479,57 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
                 corr = ex2(m_ref - m_new);
                 m_ref = m_new;
                 l_run *= corr;
-                need = 1;
             }
-            corr_s[row] = corr;
+            if (__any_sync(0xffffffffu, corr != 1.f)) {
+                // ---- correct the running output (rare): the product of the page before must be done, this page's has to wait for P ----
+                // (a correction implies an earlier page)
+                alive = __all_sync(0xffffffffu, mbar_wait(&o_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort_flag, status));
+                if (!alive) break;
+                tcgen05_fence_after();
+#pragma unroll
+                for (int c0 = 0; c0 < D; c0 += 16) {
+                    uint32_t o[16];
+                    tcgen05_ld_16(lane_addr + O_COL + (uint32_t)c0, o);
+                    tcgen05_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                    tcgen05_st_16(lane_addr + O_COL + (uint32_t)c0, o);
+                }
+            }
             const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-            // (the product of the page before must have read P)
-            if (it > 0 && alive && !mbar_wait(&o_bar, (it - 1) & 1, abort_flag, status)) alive = false;
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint32_t p_row = smem_u32(Ps) + (uint32_t)((row >> 3) * 1024 + (row & 7) * 128), p_xor = (uint32_t)(row & 7);
 #pragma unroll
-            for (int c0 = 0; c0 < PAGE; c0 += 8) {
-                uint32_t packed[4];
+            for (int c0 = 0; c0 < PAGE; c0 += 32) {
+                uint32_t packed[16];
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
+                for (int j = 0; j < 32; j += 2) {
                     const float p0 = ex2(__uint_as_float(r[c0 + j]) + neg_m), p1 = ex2(__uint_as_float(r[c0 + j + 1]) + neg_m);
                     if (Q8) {
-                        const float2 f = *reinterpret_cast<const float2 *>(&vf_s[it & 1][c0 + j]);
-                        sum4[j >> 1] = fmaf(p0, f.x, fmaf(p1, f.y, sum4[j >> 1]));
+                        const float2 f = *reinterpret_cast<const float2 *>(&vf_s[it & 3][c0 + j]);
+                        sum4[(j >> 1) & 3] = fmaf(p0, f.x, fmaf(p1, f.y, sum4[(j >> 1) & 3]));
                         const __half2 h2 = __floats2half2_rn(p0, p1);
                         packed[j >> 1] = *reinterpret_cast<const uint32_t *>(&h2);
                     } else {
-                        sum4[j >> 1] += p0 + p1;
+                        sum4[(j >> 1) & 3] += p0 + p1;
                         const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
                         packed[j >> 1] = *reinterpret_cast<const uint32_t *>(&h2);
                     }
                 }
-                st_shared_16(p_row + ((((uint32_t)(c0 >> 3)) ^ p_xor) << 4), packed[0], packed[1], packed[2], packed[3]);
+                tcgen05_st_16(s_addr + (uint32_t)(c0 >> 1), packed);
             }
             l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-        } else if (Q8) {
-            // (on their way while the softmax runs)
-            if (it + 2 < n_it) fetch(reinterpret_cast<uint4(&)[LOADS]>(raw_k), k_pages, it + 2);
-            if (it + 1 < n_it) fetch(reinterpret_cast<uint4(&)[LOADS]>(raw_v), v_pages, it + 1);
-        } else {
-            copies_wait<0>();                        // V(it) and K(it + 1)
-            if (!whole(pg)) {
-                bool odd = false;
-#pragma unroll
-                for (int u = 0; u < LOADS; ++u) {
-                    const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
-                    const uint32_t where = vs0 + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7);
-                    const uint4 v = ld_shared_16(where);
-                    st_shared_16(where, finite_pair(v.x, 0x7f807f80u, odd), finite_pair(v.y, 0x7f807f80u, odd), finite_pair(v.z, 0x7f807f80u, odd),
-                                 finite_pair(v.w, 0x7f807f80u, odd));
-                }
-                if (odd) odd_s = 1;
-            }
+            tcgen05_wait_st();
+            tcgen05_fence_before();
+            mbar_arrive(&p_full[it & 1]);
         }
-        // V(it) and K(it + 1) are in shared memory, P is written; does any row's output have to be corrected first?
-        fence_async_smem();
-        tcgen05_fence_before();
-        const int any_need = __syncthreads_or(need);
-        if (warp >= 4) {
-            if (any_need) {
-                // (a correction implies an earlier page: its product into O must be done)
-                if (alive && !mbar_wait(&o_bar, (it - 1) & 1, abort_flag, status)) alive = false;
-                tcgen05_fence_after();
-                const float corr = corr_s[row];
-                if (__any_sync(0xffffffffu, corr != 1.f)) {
-#pragma unroll
-                    for (int c0 = 0; c0 < D; c0 += 16) {
-                        uint32_t r[16];
-                        tcgen05_ld_16(lane_addr + O_COL + (uint32_t)c0, r);
-                        tcgen05_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * corr);
-                        tcgen05_st_16(lane_addr + O_COL + (uint32_t)c0, r);
-                    }
-                    tcgen05_wait_st();
-                }
-                tcgen05_fence_before();
-                asm volatile("bar.sync 1, 128;" ::: "memory");      // warps 4-7: all rows corrected before the product
-            }
-            if (tid == ISSUER) {
-                // (the next scores first: the next softmax waits for them)
-                tcgen05_fence_after();
-                if (it + 1 < n_it) issue_qk(it + 1);
-#pragma unroll
-                for (int k2 = 0; k2 < PAGE / 16; ++k2)
-                    tcgen05_mma_f16(tmem_base + O_COL, desc_p0 + (uint64_t)((k2 * 32) >> 4), desc_v0 + (uint64_t)((k2 * 2048) >> 4), idesc_pv,
-                                    (it > 0 || k2 > 0) ? 1u : 0u);
-                tcgen05_commit(&o_bar);
-            }
-            __syncwarp();
-            // the keys' stage of this page is free (its scores were seen before the barrier), the values' once the product has read it
-            if (it + 2 < n_it) {
-                columns(it + 2);
-                if (Q8) convert(ks0 + (it & 1) * K_BYTES, reinterpret_cast<uint4(&)[LOADS]>(raw_k), false);
-                else copy_page(ks0 + (it & 1) * K_BYTES, k_pages, it + 2);
-            }
-            if (it + 1 < n_it) {
-                if (alive && !mbar_wait(&o_bar, it & 1, abort_flag, status)) alive = false;
-                if (Q8) convert(vs0, reinterpret_cast<uint4(&)[LOADS]>(raw_v), !whole(pg + 1));
-                else copy_page(vs0, v_pages, it + 1);
-            }
-            copies_commit();
-        }
+        // (the last scores were seen, and were issued behind the product two pages before: the barrier is at most a phase away)
+        if (n_it > 0 && alive && !mbar_wait(&o_done[(n_it - 1) & 1], ((n_it - 1) >> 1) & 1, abort_flag, status)) alive = false;
+        fin[row][0] = m_ref, fin[row][1] = l_run;
     }
-    if (n_it > 0 && alive && !mbar_wait(&o_bar, (n_it - 1) & 1, abort_flag, status)) alive = false;
-    if (warp < 4) fin[row][0] = m_ref, fin[row][1] = l_run;
     copies_wait<0>();
-    tcgen05_fence_after();
     __syncthreads();
+    tcgen05_fence_after();
+    alive = abort_s == 0;
 
     // ---- the result: every thread half the columns of its row ----
     float *merge = reinterpret_cast<float *>(base);          // [ROWS][D + 2], where the operands were
@@ -566,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
 
 template <int D, bool Q8, typename... Args>
 int launch(dim3 grid, int cluster, cudaStream_t stream, Args... args) {
-    constexpr size_t smem = (size_t)(D / 64) * (ROWS + 3 * PAGE) * 128 + ROWS * 128 + 1024;
+    constexpr size_t smem = (size_t)(D / 64) * (ROWS + 4 * PAGE) * 128 + 1024;
     cudaError_t e = cudaFuncSetAttribute(tree_attention_tall_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) LGML_FAIL("tree_attention: cannot have %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     lgml_launch_cluster(tree_attention_tall_kernel<D, Q8>, grid, THREADS, smem, stream, cluster, args...);
