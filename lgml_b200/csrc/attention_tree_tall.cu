@@ -1,18 +1,19 @@
 // Attention of the new tokens of a request over its paged cache (attention_tree.cu has the definition) where a KV head has many rows: tokens x heads
 // of 33 and more.  There the products are what takes time, so they are on tcgen05, 128 rows a block:
 //     S[128, 64] = Q[128, D] . K_page^T        O[128, D] += P[128, 64] . V_page        accumulators in tensor memory
-// Warps 0-3 do the softmax, a thread a row, and write P back into tensor memory, over the scores it came from; warps 4-6 bring the pages, into two stages
-// of keys and of values; the first thread of warp 7 issues the products.  There are two buffers of scores: those of page it + 2 are issued behind the P V
-// product of page it, which read the buffer they go to, so a page's scores are there before the softmax of the page ahead of it is done, and the
-// only chain is softmax after softmax.  (Products of one thread complete in the order of issue.)  Operands lie in shared memory in rows of 128 bytes,
-// swizzled; V is the N-major operand.  The running output stays in tensor memory; the softmax threads correct it only when a row's maximum
-// has grown by more than 2^8 since its sums'.
+// Warps 0-7 do the softmax, two threads a row (half a page's columns each; they tell one another their maxima), and write P back into tensor memory, over the
+// scores it came from; warps 8 and 9 bring the keys, 10 and 11 the values, into two stages each; the first thread of warp 12 issues the products.  There are
+// two buffers of scores: those of page it + 2 are issued behind the P V product of page it, which read the buffer they go to, so a page's scores are there
+// before the softmax of the page ahead of it is done, and the only chain is softmax after softmax.  (Products of one thread complete in the order of
+// issue.)  Operands lie in shared memory in rows of 128 bytes, swizzled; V is the N-major operand.  The running output stays in tensor
+// memory; the softmax threads correct it only when a row's maximum has grown by more than 2^8 since its sums'.
 // Every mbarrier is of one parity of pages, and what its next phase needs comes after its waiters have seen this one, so none is missed.
 // Tensor memory is taken behind the wait for the kernels ahead, so it is never held against one of them, and the kernels behind start when this one is done.
 //
-// Pages of e4m3 become float16 on the way to shared memory, exactly: 16 codes a load, converted by the threads that load them while the
-// softmax of the page before runs.  Their powers of two stay outside: a key's multiplies its column of scores, a value's joins its column's
-// exponent, and q is scaled row by row, as in attention_tree.cu.  Pages in bfloat16 are copied as they are, a page ahead.
+// Pages of e4m3 become float16 on the way to shared memory, exactly: 16 codes a load, a page ahead in registers, converted by the threads that loaded
+// them.  Their powers of two stay outside: a key's multiplies its column of scores, a value's joins its column's
+// exponent, and q is scaled row by row, as in attention_tree.cu (a row whose largest entry is
+// between 2^-2 and 2^15 stays as it is: what float16 then rounds is under 2^-23 of that).  Pages in bfloat16 are copied as they are, a page ahead.
 //
 // Every column that a row may not see is a bit of a 64-bit word, tested only in pages that some row does not see whole.  There, values that are
 // not finite become zeros before the product (0 x NaN), and are added at the end to the rows that see them.
@@ -23,9 +24,10 @@ LGML_DEFINE_LAST_ERROR(lgml_attention_tree_tall)
 
 namespace {
 constexpr int ROWS = 128;
-constexpr int THREADS = 256;
-constexpr int LOADERS = 96;                  // threads of warps 4-6
-constexpr int ISSUER = 224;                  // the first thread of warp 7
+constexpr int THREADS = 416;
+constexpr int SOFTMAX = 256;                 // threads of warps 0-7
+constexpr int LOADERS = 64;                  // threads that bring the keys, and the values
+constexpr int KEYS = 256, VALUES = 320, ISSUER = 384;        // first thread of warps 8, 10 and 12
 constexpr uint32_t SPIN_LIMIT = 1u << 20;    // polls of up to WAIT_HINT_NS each: about a second
 constexpr uint32_t WAIT_HINT_NS = 1000;
 constexpr int STATUS_TIMEOUT = 14;
@@ -131,6 +133,23 @@ __host__ __device__ constexpr uint32_t make_idesc(int m, int n, int b_n_major, i
 // byte offset of 16-byte chunk `chunk` (0..7) of row `row` inside a swizzled block of 128-byte rows
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4)); }
 
+// two float32 products-and-sums, products, or sums, in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+
 // A pair of numbers that are not finite becomes zeros, and `odd` says so.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t x, uint32_t inf, bool &odd) {
     const uint32_t lo = inf & 0xffffu, hi = inf & 0xffff0000u;
@@ -149,12 +168,14 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     constexpr int KB = D / 64;                        // 64-element blocks along the head
     constexpr uint32_t Q_BYTES = KB * ROWS * 128, K_BYTES = KB * PAGE * 128;
     constexpr int HALF = D / 2;
-    constexpr int SIZE = Q8 ? 1 : 2, PER_ROW = D * SIZE / 16, CHUNKS = PAGE * PER_ROW, LOADS = (CHUNKS + LOADERS - 1) / LOADERS;       // 16-byte loads of a page's keys: a row's, all, a thread's
+    constexpr int SIZE = Q8 ? 1 : 2, PER_ROW = D * SIZE / 16, LOADS = PAGE * PER_ROW / LOADERS;       // 16-byte loads of a page's keys: a row's, a thread's
+    constexpr int STEP = LOADERS / PER_ROW;           // rows from one load of a thread to its next: 4, 8 or 16
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *Qs = base, *Ks = Qs + Q_BYTES, *Vs = Ks + 2 * K_BYTES;         // two stages of keys, two of values
-    __shared__ __align__(16) float2 col_s[4][PAGE];       // per column of page it (it % 4): its scores' factor, what is added to them
-    __shared__ __align__(16) float vf_s[4][PAGE];         // and what its probability counts for in the sum
+    __shared__ __align__(16) float kf_s[4][PAGE], add_s[4][PAGE], vf_s[4][PAGE];      // per column of page it (it % 4): its scores' factor, what is added to them,
+                                                                                      // and what its probability counts for in the sum
+    __shared__ float max_s[2][2][ROWS], sum_s[2][ROWS];   // by the page's parity and the half: a row's maximum; its sum, at the end
     __shared__ __align__(8) float fin[ROWS][2];
     __shared__ float unscale_s[ROWS];
     __shared__ uint64_t k_full[2], v_full[2], s_full[2], p_full[2], o_done[2];        // by the page's parity
@@ -172,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
         return;
     }
     // ---- this thread's row ----
-    const int quarter = warp & 3, row = quarter * 32 + lane;                     // (tensor memory: a warp reads its quarter of the lanes)
+    const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane;         // (tensor memory: a warp reads its quarter of the lanes)
     const bool row_valid = r0 + row < n_rows;
     const int my_tok = min(r0 + row, n_rows - 1) / group;
     const int my_pos = early_int(positions + row0 + my_tok);
@@ -209,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
             mbar_init(&k_full[i], LOADERS);
             mbar_init(&v_full[i], LOADERS);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], ROWS);
+            mbar_init(&p_full[i], SOFTMAX);
             mbar_init(&o_done[i], 1);
         }
         abort_s = odd_s = 0;
@@ -235,8 +256,8 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
                 }
 #pragma unroll
                 for (int o = CH / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));       // (CH neighbouring threads have a row)
-                // 2^x so that amax 2^x is in [2^14, 2^15)
-                const int x = min(max(14 - ((int)(__float_as_uint(amax) >> 23) - 127), -114), 100);
+                // 2^x so that amax 2^x is in [2^14, 2^15), unless it is well within float16 already
+                const int e = (int)(__float_as_uint(amax) >> 23) - 127, x = e >= -2 && e <= 14 ? 0 : min(max(14 - e, -114), 100);
                 const float up = power_of_two(x);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -258,45 +279,47 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     const float scale_log2 = scale * 1.4426950408889634f;
     bool alive = true;
 
-    // ---- the pages: warps 4-6 ----
-    const int l = tid - ROWS;                // (of 96)
+    // ---- the pages ----
+    const int l = tid & (LOADERS - 1);
     auto page_of = [&](int it) {
-        const int page = pb + it < max_blocks ? early_int(block_table + (size_t)s * max_blocks + pb + it) : -1;
+        const int page = it < n_it && pb + it < max_blocks ? early_int(block_table + (size_t)s * max_blocks + pb + it) : -1;
         return page >= 0 && page < n_pages ? page : -1;
     };
-    // Load u of a thread: chunk l + 96 u of the page, 16 bytes of row chunk / PER_ROW.
+    // Load u of a thread: 16 bytes from chunk l % PER_ROW of row l / PER_ROW + STEP u on.
+    const int l_row = l / PER_ROW, l_chunk = l - l_row * PER_ROW;
+    // Where 16-byte chunk `chunk` of that row lies in a stage.
+    auto place = [&](int chunk, int u) -> uint32_t {
+        const int r = l_row + STEP * u;
+        return (uint32_t)((chunk >> 3) * (PAGE * 128)) + swz(r, chunk & 7);
+    };
     auto fetch = [&](uint4 (&raw)[LOADS], const uint8_t *pages, int it, int page) {
         const int left = n_cells - (pb + it) * PAGE;
         const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D;
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u;
-            raw[u] = page >= 0 && at < CHUNKS && at / PER_ROW < left ? __ldcg(reinterpret_cast<const uint4 *>(src) + at) : make_uint4(0, 0, 0, 0);
-        }
+        for (int u = 0; u < LOADS; ++u)
+            raw[u] = page >= 0 && l_row + STEP * u < left ? __ldcg(reinterpret_cast<const uint4 *>(src) + l + LOADERS * u) : make_uint4(0, 0, 0, 0);
     };
     // ... as float16 in shared memory; in a page that not every row sees whole (check), without what is not finite.
     auto convert = [&](uint32_t dst, const uint4 (&raw)[LOADS], bool check) {
         bool odd = false;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u, r = at / PER_ROW, ch = 2 * (at - r * PER_ROW);
-            if (at >= CHUNKS) break;
             const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
             uint32_t h[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                h[j] = half2_of_codes((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
-                if (check) h[j] = finite_pair(h[j], 0x7c007c00u, odd);
+            for (int j = 0; j < 8; ++j) h[j] = half2_of_codes((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+            if (check) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = finite_pair(h[j], 0x7c007c00u, odd);
             }
-            const uint32_t block = dst + (ch >> 3) * (PAGE * 128);
-            st_shared_16(block + swz(r, ch & 7), h[0], h[1], h[2], h[3]);
-            st_shared_16(block + swz(r, (ch & 7) + 1), h[4], h[5], h[6], h[7]);
+            st_shared_16(dst + place(2 * l_chunk, u), h[0], h[1], h[2], h[3]);
+            st_shared_16(dst + place(2 * l_chunk + 1, u), h[4], h[5], h[6], h[7]);
         }
         if (odd) odd_s = 1;
     };
     // What the softmax of page it has to know of its columns: the exponents of column l, as bytes ...
     auto exponents = [&](int it, int page) -> int2 {
-        if (!Q8 || l >= PAGE || page < 0 || (pb + it) * PAGE + l >= n_cells) return make_int2(127, 127);
+        if (!Q8 || page < 0 || (pb + it) * PAGE + l >= n_cells) return make_int2(127, 127);
         const size_t vec = ((size_t)page * Hkv + kvh) * PAGE + l;
         return make_int2((int)__ldcg(k_exps + vec), (int)__ldcg(v_exps + vec));
     };
@@ -304,101 +327,81 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     auto columns = [&](int it, int page, int2 e) {
         if (l == 0) ok_s[it & 3] = page >= 0;
         if (l == 0 && page < 0) atomicExch(status, 3);
-        if (Q8 && l < PAGE) {
+        if (Q8) {
             const int ke = min(e.x, 246) - 127, ve = min(e.y, 246) - 127;
-            col_s[it & 3][l] = make_float2(scale_log2 * power_of_two(ke), (float)ve);
+            kf_s[it & 3][l] = scale_log2 * power_of_two(ke);
+            add_s[it & 3][l] = (float)ve;
             vf_s[it & 3][l] = power_of_two(-ve);
         }
     };
-    // bfloat16: asynchronous copies
+    // bfloat16: asynchronous copies, and what they will need two pages on asked of L2
     auto copy_page = [&](uint32_t dst, const uint8_t *pages, int it, int page) {
         const int left = n_cells - (pb + it) * PAGE;
         const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D * 2;
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
-            if (at < CHUNKS) copy_16(dst + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7), src + (size_t)at * 16, page >= 0 && r < left);
-        }
+        for (int u = 0; u < LOADS; ++u) copy_16(dst + place(l_chunk, u), src + (size_t)(l + LOADERS * u) * 16, page >= 0 && l_row + STEP * u < left);
+        copies_commit();
+    };
+    auto ask_l2 = [&](const uint8_t *pages, int page) {
+        if (page < 0) return;
+        const uint8_t *src = pages + ((size_t)page * Hkv + kvh) * PAGE * D * 2;
+#pragma unroll
+        for (int u = 0; u < PAGE * D * 2 / 128 / LOADERS; ++u) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (size_t)(l + LOADERS * u) * 128));
     };
     const uint32_t ks0 = smem_u32(Ks), vs0 = smem_u32(Vs);
     float m_ref = -INFINITY, l_run = 0.f;
-    if (warp >= 4 && warp < 7) {
-        // page it's stage is free when the products of page it - 2 have read it
-        auto wait_for = [&](uint64_t *bar, int it) {
-            if (it >= 2 && alive && !mbar_wait(&bar[it & 1], ((it - 2) >> 1) & 1, abort_flag, status)) alive = false;
-        };
+    if (tid >= KEYS && tid < ISSUER) {
+        // ---- the keys, or the values: page it's stage is free when the products of page it - 2 have read it ----
         // (page numbers come two pages ahead, codes and exponents one: each is a trip to L2 or beyond)
-        int page = n_it > 0 ? page_of(0) : -1, page1 = n_it > 1 ? page_of(1) : -1;
-        if (Q8) {
-            uint4 raw_k[LOADS], raw_v[LOADS];
-            int2 exps = make_int2(127, 127);
-            if (n_it > 0) {
-                exps = exponents(0, page);
-                fetch(raw_k, k_pages, 0, page);
-                fetch(raw_v, v_pages, 0, page);
-            }
-            for (int it = 0; it < n_it && alive; ++it) {
-                const int page2 = it + 2 < n_it ? page_of(it + 2) : -1;
-                wait_for(s_full, it);
-                columns(it, page, exps);
-                convert(ks0 + (it & 1) * K_BYTES, raw_k, false);
-                fence_async_smem();
-                mbar_arrive(&k_full[it & 1]);
-                if (it + 1 < n_it) {
-                    exps = exponents(it + 1, page1);
-                    fetch(raw_k, k_pages, it + 1, page1);
-                }
-                wait_for(o_done, it);
-                convert(vs0 + (it & 1) * K_BYTES, raw_v, !whole(pb + it));
-                fence_async_smem();
-                mbar_arrive(&v_full[it & 1]);
-                if (it + 1 < n_it) fetch(raw_v, v_pages, it + 1, page1);
-                page = page1, page1 = page2;
-            }
-        } else {
-            // (a page's keys are asked for, then the page before is handed on, then this one's values are asked for: they wait for the product of
-            //  two pages before, which waits for that page)
-            for (int it = 0; it <= n_it && alive; ++it) {
-                const int page2 = it + 2 < n_it ? page_of(it + 2) : -1;
-                if (it < n_it) {
-                    wait_for(s_full, it);
-                    columns(it, page, make_int2(127, 127));
-                    copy_page(ks0 + (it & 1) * K_BYTES, k_pages, it, page);
-                }
-                copies_commit();
-                auto values = [&]() {
-                    if (it < n_it) {
-                        wait_for(o_done, it);
-                        copy_page(vs0 + (it & 1) * K_BYTES, v_pages, it, page);
+        const bool keys = tid < VALUES;
+        const uint8_t *pages = keys ? k_pages : v_pages;
+        const uint32_t stages = keys ? ks0 : vs0;
+        uint64_t *full = keys ? k_full : v_full, *read = keys ? s_full : o_done;
+        int page = page_of(0), page1 = page_of(1);
+        uint4 raw[Q8 ? LOADS : 1];
+        int2 exps = make_int2(127, 127);
+        if (Q8 && n_it > 0) {
+            if (keys) exps = exponents(0, page);
+            fetch(reinterpret_cast<uint4(&)[LOADS]>(raw), pages, 0, page);
+        }
+        // (bfloat16: a page is handed on when the next one has been asked for)
+        for (int it = 0; it < n_it + (Q8 ? 0 : 1) && alive; ++it) {
+            const int page2 = page_of(it + 2);
+            if (it < n_it) {
+                if (it >= 2 && !mbar_wait(&read[it & 1], ((it - 2) >> 1) & 1, abort_flag, status)) break;
+                if (keys) columns(it, page, exps);
+                if (Q8) {
+                    convert(stages + (it & 1) * K_BYTES, reinterpret_cast<uint4(&)[LOADS]>(raw), !keys && !whole(pb + it));
+                    fence_async_smem();
+                    mbar_arrive(&full[it & 1]);
+                    if (it + 1 < n_it) {
+                        if (keys) exps = exponents(it + 1, page1);
+                        fetch(reinterpret_cast<uint4(&)[LOADS]>(raw), pages, it + 1, page1);
                     }
-                    copies_commit();
-                    page = page1, page1 = page2;
-                };
-                if (it == 0) {
-                    values();
-                    continue;
+                } else {
+                    copy_page(stages + (it & 1) * K_BYTES, pages, it, page);
+                    ask_l2(pages, page2);
                 }
-                copies_wait<1>();               // all but the keys just asked for
+            }
+            if (!Q8 && it > 0) {
                 const int pr = it - 1;
-                fence_async_smem();
-                mbar_arrive(&k_full[pr & 1]);
-                if (!whole(pb + pr)) {
+                if (it < n_it) copies_wait<1>();
+                else copies_wait<0>();
+                if (!keys && !whole(pb + pr)) {
                     bool odd = false;
 #pragma unroll
                     for (int u = 0; u < LOADS; ++u) {
-                        const int at = l + LOADERS * u, r = at / PER_ROW, ch = at - r * PER_ROW;
-                        if (at >= CHUNKS) break;
-                        const uint32_t where = vs0 + (pr & 1) * K_BYTES + (ch >> 3) * (PAGE * 128) + swz(r, ch & 7);
+                        const uint32_t where = vs0 + (pr & 1) * K_BYTES + place(l_chunk, u);
                         const uint4 v = ld_shared_16(where);
                         st_shared_16(where, finite_pair(v.x, 0x7f807f80u, odd), finite_pair(v.y, 0x7f807f80u, odd), finite_pair(v.z, 0x7f807f80u, odd),
                                      finite_pair(v.w, 0x7f807f80u, odd));
                     }
                     if (odd) odd_s = 1;
-                    fence_async_smem();
                 }
-                mbar_arrive(&v_full[pr & 1]);
-                values();
+                fence_async_smem();
+                mbar_arrive(&full[pr & 1]);
             }
+            page = page1, page1 = page2;
         }
     } else if (tid == ISSUER) {
         // ---- the products ----
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
         }
         for (int it = 0; it < n_it && alive; ++it) {
             const uint32_t ph = (it >> 1) & 1;
-            alive = mbar_wait(&p_full[it & 1], ph, abort_flag, status) && mbar_wait(&v_full[it & 1], ph, abort_flag, status);
+            alive = mbar_wait(&v_full[it & 1], ph, abort_flag, status) && mbar_wait(&p_full[it & 1], ph, abort_flag, status);
             tcgen05_fence_after();
             if (!alive) break;
             const uint64_t dv = desc_v0 + (uint64_t)(((it & 1) * K_BYTES) >> 4);
@@ -436,42 +439,55 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
                 if (alive) issue_scores(it + 2);
             }
         }
-    } else if (warp < 4) {
-        // ---- softmax ----
+    } else if (tid < SOFTMAX) {
+        // ---- softmax: columns 32 half .. 32 half + 31 of this row ----
+        constexpr int COLS = PAGE / 2;
+        const int c_first = half * COLS;
         const float unscale = Q8 ? unscale_s[row] : 1.f;
+        const bool any_scaled = Q8 && __any_sync(0xffffffffu, unscale != 1.f);
         for (int it = 0; it < n_it; ++it) {
             const int pg = pb + it;
             const uint32_t s_addr = lane_addr + (uint32_t)(it & 1) * S1_COL;
-            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[it & 1], (it >> 1) & 1, abort_flag, status));         // (a warp goes on, or stops, as one)
-            if (!alive) break;
+            // (a warp gives up as one, and then goes through its pages without waiting: its partner meets it in each)
+            alive = __all_sync(0xffffffffu, alive && mbar_wait(&s_full[it & 1], (it >> 1) & 1, abort_flag, status));
             tcgen05_fence_after();
-            const bool edge = !whole(pg) || !ok_s[it & 3];
-            uint32_t r[PAGE];
-#pragma unroll
-            for (int c0 = 0; c0 < PAGE; c0 += 16) tcgen05_ld_16(s_addr + (uint32_t)c0, *reinterpret_cast<uint32_t(*)[16]>(&r[c0]));
+            const bool there = ok_s[it & 3] != 0, edge = !whole(pg) || !there;
+            union {
+                uint32_t u[COLS];
+                float2 f[COLS / 2];
+            } r;
+            tcgen05_ld_16(s_addr + (uint32_t)c_first, *reinterpret_cast<uint32_t(*)[16]>(&r.u[0]));
+            tcgen05_ld_16(s_addr + (uint32_t)c_first + 16u, *reinterpret_cast<uint32_t(*)[16]>(&r.u[16]));
             tcgen05_wait_ld();
             if (Q8) {
+                if (any_scaled) {
 #pragma unroll
-                for (int c = 0; c < PAGE; c += 2) {
-                    const float4 f = *reinterpret_cast<const float4 *>(&col_s[it & 3][c]);
-                    r[c] = __float_as_uint(fmaf(__uint_as_float(r[c]) * unscale, f.x, f.y));
-                    r[c + 1] = __float_as_uint(fmaf(__uint_as_float(r[c + 1]) * unscale, f.z, f.w));
+                    for (int c = 0; c < COLS / 2; ++c) r.f[c] = mul2(r.f[c], make_float2(unscale, unscale));
+                }
+#pragma unroll
+                for (int c = 0; c < COLS; c += 4) {
+                    const float4 kf = *reinterpret_cast<const float4 *>(&kf_s[it & 3][c_first + c]), ad = *reinterpret_cast<const float4 *>(&add_s[it & 3][c_first + c]);
+                    r.f[c / 2] = fma2(r.f[c / 2], make_float2(kf.x, kf.y), make_float2(ad.x, ad.y));
+                    r.f[c / 2 + 1] = fma2(r.f[c / 2 + 1], make_float2(kf.z, kf.w), make_float2(ad.z, ad.w));
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < PAGE; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * scale_log2);
+                for (int c = 0; c < COLS / 2; ++c) r.f[c] = mul2(r.f[c], make_float2(scale_log2, scale_log2));
             }
             if (edge) {
-                const unsigned long long v = ok_s[it & 3] ? seen_of(pg) : 0ull;
-                const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+                const uint32_t v = there ? (uint32_t)(seen_of(pg) >> c_first) : 0u;
 #pragma unroll
-                for (int c = 0; c < PAGE; ++c)
-                    if (!(((c < 32 ? lo : hi) >> (c & 31)) & 1u)) r[c] = __float_as_uint(-INFINITY);
+                for (int c = 0; c < COLS; ++c)
+                    if (!((v >> c) & 1u)) r.u[c] = __float_as_uint(-INFINITY);
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < PAGE; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(r[c]));
-            const float m_new = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            for (int c = 0; c < COLS; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(r.u[c]));
+            const float mine = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            // the row's other thread is in the warp four further: the two warps meet here.  (Behind this both have their scores, so P may be written over them.)
+            max_s[it & 1][half][row] = mine;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+            const float m_new = fmaxf(mine, max_s[it & 1][half ^ 1][row]);
             float corr = 1.f;
             if (m_ref == -INFINITY) {
                 m_ref = m_new;                       // nothing summed yet: nothing to correct
@@ -481,61 +497,58 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
                 l_run *= corr;
             }
             if (__any_sync(0xffffffffu, corr != 1.f)) {
-                // ---- correct the running output (rare): the product of the page before must be done, this page's has to wait for P ----
+                // ---- correct this half of the running output (rare): the product of the page before must be done, this page's has to wait for P ----
                 // (a correction implies an earlier page)
-                alive = __all_sync(0xffffffffu, mbar_wait(&o_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort_flag, status));
-                if (!alive) break;
+                alive = __all_sync(0xffffffffu, alive && mbar_wait(&o_done[(it - 1) & 1], ((it - 1) >> 1) & 1, abort_flag, status));
                 tcgen05_fence_after();
 #pragma unroll
-                for (int c0 = 0; c0 < D; c0 += 16) {
+                for (int c0 = 0; c0 < HALF; c0 += 16) {
                     uint32_t o[16];
-                    tcgen05_ld_16(lane_addr + O_COL + (uint32_t)c0, o);
+                    tcgen05_ld_16(lane_addr + O_COL + (uint32_t)(half * HALF + c0), o);
                     tcgen05_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                    tcgen05_st_16(lane_addr + O_COL + (uint32_t)c0, o);
+                    tcgen05_st_16(lane_addr + O_COL + (uint32_t)(half * HALF + c0), o);
                 }
             }
             const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t packed[16];
 #pragma unroll
-            for (int c0 = 0; c0 < PAGE; c0 += 32) {
-                uint32_t packed[16];
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float p0 = ex2(__uint_as_float(r[c0 + j]) + neg_m), p1 = ex2(__uint_as_float(r[c0 + j + 1]) + neg_m);
-                    if (Q8) {
-                        const float2 f = *reinterpret_cast<const float2 *>(&vf_s[it & 3][c0 + j]);
-                        sum4[(j >> 1) & 3] = fmaf(p0, f.x, fmaf(p1, f.y, sum4[(j >> 1) & 3]));
-                        const __half2 h2 = __floats2half2_rn(p0, p1);
-                        packed[j >> 1] = *reinterpret_cast<const uint32_t *>(&h2);
-                    } else {
-                        sum4[(j >> 1) & 3] += p0 + p1;
-                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-                        packed[j >> 1] = *reinterpret_cast<const uint32_t *>(&h2);
-                    }
+            for (int c = 0; c < COLS / 2; ++c) {
+                const float2 x = add2(r.f[c], make_float2(neg_m, neg_m)), e = make_float2(ex2(x.x), ex2(x.y));
+                if (Q8) {
+                    sum2[c & 1] = fma2(e, *reinterpret_cast<const float2 *>(&vf_s[it & 3][c_first + 2 * c]), sum2[c & 1]);
+                    const __half2 h2 = __floats2half2_rn(e.x, e.y);
+                    packed[c] = *reinterpret_cast<const uint32_t *>(&h2);
+                } else {
+                    sum2[c & 1] = add2(sum2[c & 1], e);
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(e.x, e.y);
+                    packed[c] = *reinterpret_cast<const uint32_t *>(&h2);
                 }
-                tcgen05_st_16(s_addr + (uint32_t)(c0 >> 1), packed);
             }
-            l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            tcgen05_st_16(s_addr + (uint32_t)(c_first >> 1), packed);
+            l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
             tcgen05_wait_st();
             tcgen05_fence_before();
             mbar_arrive(&p_full[it & 1]);
         }
         // (the last scores were seen, and were issued behind the product two pages before: the barrier is at most a phase away)
         if (n_it > 0 && alive && !mbar_wait(&o_done[(n_it - 1) & 1], ((n_it - 1) >> 1) & 1, abort_flag, status)) alive = false;
-        fin[row][0] = m_ref, fin[row][1] = l_run;
+        sum_s[half][row] = l_run;
+        if (half == 0) fin[row][0] = m_ref;
     }
     copies_wait<0>();
     __syncthreads();
     tcgen05_fence_after();
     alive = abort_s == 0;
+    if (tid < ROWS) fin[row][1] = sum_s[0][row] + sum_s[1][row];
 
     // ---- the result: every thread half the columns of its row ----
     float *merge = reinterpret_cast<float *>(base);          // [ROWS][D + 2], where the operands were
-    {
-        const float M = fin[row][0], sum = fin[row][1];
-        const int col0 = warp < 4 ? 0 : HALF;
+    if (tid < SOFTMAX) {
+        const float M = fin[row][0], sum = sum_s[0][row] + sum_s[1][row];
+        const int col0 = half * HALF;
         __nv_bfloat16 *dst = row_at(out, ldo, row0, min(r0 + row, n_rows - 1), group, kvh, D, 0);
         const size_t part = ((size_t)(row0 + my_tok) * H + kvh * group + min(r0 + row, n_rows - 1) % group) * n_splits + split;
         const bool odd = odd_s != 0;
