@@ -42,6 +42,11 @@ __device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t a, uint32_t
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// A whole warp's: one arrival for its 32 threads (each would be an operation of its own on the barrier, one after the other).
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -227,10 +232,10 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], LOADERS);
-            mbar_init(&v_full[i], LOADERS);
+            mbar_init(&k_full[i], LOADERS / 32);
+            mbar_init(&v_full[i], LOADERS / 32);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], SOFTMAX);
+            mbar_init(&p_full[i], SOFTMAX / 32);
             mbar_init(&o_done[i], 1);
         }
         abort_s = odd_s = 0;
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
             vf_s[it & 3][l] = power_of_two(-ve);
         }
     };
-    // bfloat16: asynchronous copies, and what they will need two pages on asked of L2
+    // bfloat16: asynchronous copies
     auto copy_page = [&](uint32_t dst, const uint8_t *pages, int it, int page) {
         const int left = n_cells - (pb + it) * PAGE;
         const uint8_t *src = pages + ((size_t)max(page, 0) * Hkv + kvh) * PAGE * D * 2;
@@ -344,54 +349,60 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
     };
     auto ask_l2 = [&](const uint8_t *pages, int page) {
         if (page < 0) return;
-        const uint8_t *src = pages + ((size_t)page * Hkv + kvh) * PAGE * D * 2;
+        const uint8_t *src = pages + ((size_t)page * Hkv + kvh) * PAGE * D * SIZE;
 #pragma unroll
-        for (int u = 0; u < PAGE * D * 2 / 128 / LOADERS; ++u) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (size_t)(l + LOADERS * u) * 128));
+        for (int u = 0; u < (PAGE * D * SIZE / 128 + LOADERS - 1) / LOADERS; ++u)
+            if (l + LOADERS * u < PAGE * D * SIZE / 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (size_t)(l + LOADERS * u) * 128));
     };
     const uint32_t ks0 = smem_u32(Ks), vs0 = smem_u32(Vs);
     float m_ref = -INFINITY, l_run = 0.f;
     if (tid >= KEYS && tid < ISSUER) {
         // ---- the keys, or the values: page it's stage is free when the products of page it - 2 have read it ----
-        // (page numbers come two pages ahead, codes and exponents one: each is a trip to L2 or beyond)
+        // (page numbers come four pages ahead and ask L2 for their pages, codes and exponents one page ahead: each is a trip to L2 or beyond)
         const bool keys = tid < VALUES;
         const uint8_t *pages = keys ? k_pages : v_pages;
         const uint32_t stages = keys ? ks0 : vs0;
         uint64_t *full = keys ? k_full : v_full, *read = keys ? s_full : o_done;
-        int page = page_of(0), page1 = page_of(1);
-        uint4 raw[Q8 ? LOADS : 1];
-        int2 exps = make_int2(127, 127);
-        if (Q8 && n_it > 0) {
-            if (keys) exps = exponents(0, page);
-            fetch(reinterpret_cast<uint4(&)[LOADS]>(raw), pages, 0, page);
-        }
-        // (bfloat16: a page is handed on when the next one has been asked for)
-        for (int it = 0; it < n_it + (Q8 ? 0 : 1) && alive; ++it) {
-            const int page2 = page_of(it + 2);
-            if (it < n_it) {
-                if (it >= 2 && !mbar_wait(&read[it & 1], ((it - 2) >> 1) & 1, abort_flag, status)) break;
-                if (keys) columns(it, page, exps);
-                if (Q8) {
-                    convert(stages + (it & 1) * K_BYTES, reinterpret_cast<uint4(&)[LOADS]>(raw), !keys && !whole(pb + it));
-                    fence_async_smem();
-                    mbar_arrive(&full[it & 1]);
-                    if (it + 1 < n_it) {
-                        if (keys) exps = exponents(it + 1, page1);
-                        fetch(reinterpret_cast<uint4(&)[LOADS]>(raw), pages, it + 1, page1);
-                    }
-                } else {
-                    copy_page(stages + (it & 1) * K_BYTES, pages, it, page);
-                    ask_l2(pages, page2);
-                }
+        int next[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = page_of(i);
+#pragma unroll
+        for (int i = Q8 ? 1 : 2; i < 4; ++i) ask_l2(pages, next[i]);
+        if (Q8) {
+            uint4 raw[LOADS];
+            int2 exps = make_int2(127, 127);
+            if (n_it > 0) {
+                if (keys) exps = exponents(0, next[0]);
+                fetch(raw, pages, 0, next[0]);
             }
-            if (!Q8 && it > 0) {
-                const int pr = it - 1;
-                if (it < n_it) copies_wait<1>();
-                else copies_wait<0>();
-                if (!keys && !whole(pb + pr)) {
+            for (int it = 0; it < n_it; ++it) {
+                const int coming = page_of(it + 4);
+                if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(&read[it & 1], ((it - 2) >> 1) & 1, abort_flag, status))) break;
+                if (keys) columns(it, next[0], exps);
+                convert(stages + (it & 1) * K_BYTES, raw, !keys && !whole(pb + it));
+                fence_async_smem();
+                warp_arrive(&full[it & 1]);
+                if (it + 1 < n_it) {
+                    if (keys) exps = exponents(it + 1, next[1]);
+                    fetch(raw, pages, it + 1, next[1]);
+                }
+                next[0] = next[1], next[1] = next[2], next[2] = next[3], next[3] = coming;
+                ask_l2(pages, coming);
+            }
+        } else {
+            for (int it = 0; it < 2; ++it) {
+                if (it < n_it) copy_page(stages + it * K_BYTES, pages, it, next[it]);
+                else copies_commit();
+            }
+            for (int it = 0; it < n_it; ++it) {
+                const int coming = page_of(it + 4);
+                if (keys) columns(it, next[0], make_int2(127, 127));
+                copies_wait<1>();
+                if (!keys && !whole(pb + it)) {
                     bool odd = false;
 #pragma unroll
                     for (int u = 0; u < LOADS; ++u) {
-                        const uint32_t where = vs0 + (pr & 1) * K_BYTES + place(l_chunk, u);
+                        const uint32_t where = vs0 + (it & 1) * K_BYTES + place(l_chunk, u);
                         const uint4 v = ld_shared_16(where);
                         st_shared_16(where, finite_pair(v.x, 0x7f807f80u, odd), finite_pair(v.y, 0x7f807f80u, odd), finite_pair(v.z, 0x7f807f80u, odd),
                                      finite_pair(v.w, 0x7f807f80u, odd));
@@ -399,9 +410,17 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
                     if (odd) odd_s = 1;
                 }
                 fence_async_smem();
-                mbar_arrive(&full[pr & 1]);
+                warp_arrive(&full[it & 1]);
+                // the stage is free again when this page's products have read it: the page after the next
+                if (it + 2 < n_it) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&read[it & 1], (it >> 1) & 1, abort_flag, status))) break;
+                    copy_page(stages + (it & 1) * K_BYTES, pages, it + 2, next[2]);
+                } else {
+                    copies_commit();
+                }
+                next[0] = next[1], next[1] = next[2], next[2] = next[3], next[3] = coming;
+                ask_l2(pages, coming);
             }
-            page = page1, page1 = page2;
         }
     } else if (tid == ISSUER) {
         // ---- the products ----
@@ -531,7 +550,7 @@ __global__ void __launch_bounds__(THREADS, 2) tree_attention_tall_kernel(
             l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
             tcgen05_wait_st();
             tcgen05_fence_before();
-            mbar_arrive(&p_full[it & 1]);
+            warp_arrive(&p_full[it & 1]);
         }
         // (the last scores were seen, and were issued behind the product two pages before: the barrier is at most a phase away)
         if (n_it > 0 && alive && !mbar_wait(&o_done[(n_it - 1) & 1], ((n_it - 1) >> 1) & 1, abort_flag, status)) alive = false;

@@ -22,6 +22,7 @@ _STATUS_TEXT = {
     3: "attention met a position without a page in the block table",
     10: "a tensor-core matrix product gave up waiting for its own copies or products",
     12: "the tensor-core prompt attention (one tile per CTA) gave up waiting for its own copies or products",
+    15: "the log probabilities gave up waiting for their own copies",
     14: "the attention of drafted tokens gave up waiting for its own products",
     13: "the tensor-core prompt attention (two tiles per CTA) gave up waiting for its own copies or products",
 }
