@@ -61,7 +61,6 @@ LIBRARIES: Dict[str, tuple] = {
     "kv_store": ("kv_store.cu", []),
     "attention_tree": ("attention_tree.cu", []),
     "attention_tree_tall": ("attention_tree_tall.cu", []),
-    "attention_tree_codes": ("attention_tree_codes.cu", []),
     "logprobs": ("logprobs.cu", []),
 }
 
@@ -157,7 +156,6 @@ LIBRARY_HEADERS: Dict[str, List[str]] = {
     "ssd": ["bf16_thirds.cuh"],
     "attention_tree": ["tree_common.cuh"],
     "attention_tree_tall": ["tree_common.cuh"],
-    "attention_tree_codes": ["tree_common.cuh"],
 }
 
 

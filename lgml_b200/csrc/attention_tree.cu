@@ -465,13 +465,7 @@ int launch_one(dim3 grid, int cluster, cudaStream_t stream, Args... args) {
 }
 template <int KS, bool Q8, typename... Args>
 int launch_rows(int nt, Args... args) {
-    // (up to 8 rows over pages of e4m3 with head sizes in steps of 32 are attention_tree_codes.cu's)
-    if constexpr (!Q8 || KS % 2 != 0) {
-        if (nt == 1) return launch_one<KS, 1, Q8>(args...);
-    } else if (nt == 1) {
-        LGML_FAIL("tree_attention: up to 8 rows over pages of e4m3 with head_dim %d are not handled here", 16 * KS);
-    }
-    return nt == 2 ? launch_one<KS, 2, Q8>(args...) : launch_one<KS, 4, Q8>(args...);
+    return nt == 1 ? launch_one<KS, 1, Q8>(args...) : nt == 2 ? launch_one<KS, 2, Q8>(args...) : launch_one<KS, 4, Q8>(args...);
 }
 template <bool Q8, typename... Args>
 int launch_dim(int ks, Args... args) {

@@ -2933,9 +2933,7 @@ E4M3 = torch.float8_e4m3fn
 TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
 TREE_MAX_DIM = 128
 TREE_TALL_ROWS = 33         # rows of a KV head (tokens x heads) from which it takes 128 of them a block, on tcgen05
-TREE_CODES_ROWS = 8         # ... and up to which pages of e4m3 go into the tensor cores as they are
 TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
-_TREE_NAMES = {lib: "lgml_" + lib.replace("attention_tree", "tree_attention") for lib in ("attention_tree", "attention_tree_codes", "attention_tree_tall")}
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
 
 
@@ -3070,10 +3068,10 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     _are(who, dev, torch.int32, 1, "page list, status", pages, status)
     n = pages.numel()
     shape = (n, hkv, page, d)
-    if k_out is None and v_out is None:
-        k_out, v_out = torch.empty((2,) + shape, dtype=torch.bfloat16, device=k_pages.device).unbind()
-    elif k_out is None or v_out is None:
-        raise KernelError(f"{who}: results for the keys and the values, or for neither")
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
     _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
     if k_out.shape != shape or v_out.shape != shape or status.numel() != 1:
         raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}, and the status is one int32")
@@ -3084,16 +3082,11 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
 
 
 def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64, tall: bool = False) -> int:
-    """Into how many ranges of pages ``tree_attention`` cuts a request's cells: as many as fill the SMs with its blocks, two pages at least each; up to 8 join in
-    one kernel, more cost a second one (4 us) and are taken for 128 pages and more, of eight pages each.  (``kernel_bench tree_attention``, 32 heads on 8 of 128,
-    e4m3, us: one request of 1,001 cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 51 in 8, 30 in 62; eight of
-    2,176 29, 17 in 7 and 8, 22 in 16; 16 of 4,001 59, 34 in 4, 41 in 8; 64 of up to 4,097 88, 85 in 2, 125 in 8.  With 64 drafted tokens, four requests of up
-    to 8,256 175, 70 in 4, 85 in 8.)"""
-    height, per_sm = (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
+    """Into how many ranges of pages ``tree_attention`` cuts a request's cells."""
+    height, per_sm = (128, 2) if tall else (8 if rows <= 8 else 16 if rows <= 16 else 32, 4)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
-    n = max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
-    return n if n <= TREE_CLUSTER else TREE_CLUSTER if pages < 128 else max(TREE_CLUSTER, min(n, pages // 8))
+    return max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
 
 
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
@@ -3129,7 +3122,6 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
             raise KernelError(f"{who}: one mask a token")
     rows = max_new_tokens * (n_heads // hkv)
     tall = rows >= TREE_TALL_ROWS and d in (64, 128) and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
-    codes = k_exps is not None and rows <= TREE_CODES_ROWS and d % 32 == 0
     if n_splits is None:
         n_splits = tree_splits(seqs, hkv, rows, max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page), page, tall)
     if n_splits > TREE_CLUSTER:
@@ -3139,8 +3131,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         _are(who, dev, torch.float32, 1, "scratch", scratch)
         if scratch.numel() < need:
             raise KernelError(f"{who}: scratch of {scratch.numel()} floats, {need} needed")
-    lib = "attention_tree_tall" if tall else "attention_tree_codes" if codes else "attention_tree"
-    name = _TREE_NAMES[lib]
+    lib, name = ("attention_tree_tall", "lgml_tree_attention_tall") if tall else ("attention_tree", "lgml_tree_attention")
     fn = _fn(lib, name, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
                          c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
     _check(lib, fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
@@ -3197,14 +3188,12 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: to
         raise KernelError(f"{who}: {top} alternatives (0 to min(vocabulary {v}, {LOGPROBS_TOP}))")
     # all results in one allocation, each kind in one run: log p, rank, entropy, then ids and log p of the best
     flat = torch.empty(n * (3 + 2 * top), dtype=torch.float32, device=logits.device)
-    at = flat.data_ptr()
+    at, ints = flat.data_ptr(), flat.view(torch.int32)
     fn = _fn("logprobs", "lgml_token_logprobs", [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                  c_void_p])
     _check("logprobs", fn(logits.data_ptr(), max(ld, v), n, v, ids.data_ptr(), int(top), _logprob_slices(n, v), at, at + 4 * n, at + 8 * n, at + 12 * n,
                           at + 12 * n + 4 * n * top, status.data_ptr(), _stream()), who)
-    ints, many = flat.view(torch.int32), (n, top)
-    return TokenLogprobs(flat.as_strided((n,), (1,), 0), ints.as_strided((n,), (1,), n), flat.as_strided((n,), (1,), 2 * n),
-                         ints.as_strided(many, (top, 1), 3 * n), flat.as_strided(many, (top, 1), 3 * n + n * top))
+    return TokenLogprobs(flat[:n], ints[n:2 * n], flat[2 * n:3 * n], ints[3 * n:3 * n + n * top].view(n, top), flat[3 * n + n * top:3 * n + 2 * n * top].view(n, top))
 
 
 @functools.lru_cache(maxsize=None)
