@@ -70,14 +70,14 @@ __device__ __forceinline__ void read_words(unsigned (&r)[N], const uint8_t *p) {
 // Which entries of a row a thread has, for rows of KS x 16 entries.
 //   keys: thread c = lane % 4 has, of every 4 E neighbouring entries, E: as the columns of E / 4 products
 //   values: thread g = lane / 4 has, of every 8 E neighbouring entries, E: as rows g and g + 8 of E / 2 products
-template <int KS, bool Q8> struct Cut {
+template <int KS, int NT, bool Q8> struct Cut {
     static constexpr int SIZE = Q8 ? 1 : 2;
     static constexpr int KE = Q8 ? (KS % 8 == 0 ? 32 : KS % 4 == 0 ? 16 : KS % 2 == 0 ? 8 : 4) : (KS % 4 == 0 ? 16 : KS % 2 == 0 ? 8 : 4);
     static constexpr int VE = Q8 ? (KS % 8 == 0 ? 16 : KS % 4 == 0 ? 8 : KS % 2 == 0 ? 4 : 2) : (KS % 4 == 0 ? 8 : KS % 2 == 0 ? 4 : 2);
     static constexpr int KW = KE * SIZE / 4, VW = VE * SIZE / 4;       // words of these (a value's 2 codes of e4m3: half a word)
     static constexpr int ROW = KS * 16 * SIZE, PITCH = ROW + 16;       // bytes of a row, and from row to row in a stage
     static constexpr int STAGE = 32 * PITCH + 32;                      // 16 keys, 16 values, their exponents
-    static constexpr int STAGES = 3;
+    static constexpr int STAGES = NT == 1 ? 2 : 3;                     // (one tile of rows: more blocks on an SM are worth more than a third stage)
     static __device__ __forceinline__ int key_entry(int ks, int c) { return (ks / (KE / 4)) * 4 * KE + c * KE + (ks % (KE / 4)) * 4; }
     static __device__ __forceinline__ int value_entry(int mt, int g) { return (mt / (VE / 2)) * 8 * VE + g * VE + (mt % (VE / 2)) * 2; }
 };
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     float scale, int window, int *__restrict__ status) {
     pdl_trigger();
     constexpr int D = KS * 16, ROWS = 8 * NT;
-    using C = Cut<KS, Q8>;
+    using C = Cut<KS, NT, Q8>;
     extern __shared__ __align__(16) uint8_t smem[];                // the warps' stages; at the end [WARPS][ROWS][D + 2] floats
     __shared__ int row_pos[ROWS];
     __shared__ long long row_mask[ROWS];
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 
 template <int KS, int NT, bool Q8, typename... Args>
 int launch_one(dim3 grid, int cluster, cudaStream_t stream, Args... args) {
-    using C = Cut<KS, Q8>;
+    using C = Cut<KS, NT, Q8>;
     const size_t stages = (size_t)WARPS * C::STAGES * C::STAGE, merge = sizeof(float) * WARPS * 8 * NT * (KS * 16 + 2);
     const size_t smem = stages > merge ? stages : merge;
     cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<KS, NT, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -3068,10 +3068,10 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     _are(who, dev, torch.int32, 1, "page list, status", pages, status)
     n = pages.numel()
     shape = (n, hkv, page, d)
-    if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
-    if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_pages.device)
+    if k_out is None and v_out is None:
+        k_out, v_out = torch.empty((2,) + shape, dtype=torch.bfloat16, device=k_pages.device).unbind()
+    elif k_out is None or v_out is None:
+        raise KernelError(f"{who}: results for the keys and the values, or for neither")
     _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
     if k_out.shape != shape or v_out.shape != shape or status.numel() != 1:
         raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}, and the status is one int32")
@@ -3082,11 +3082,16 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
 
 
 def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64, tall: bool = False) -> int:
-    """Into how many ranges of pages ``tree_attention`` cuts a request's cells."""
-    height, per_sm = (128, 2) if tall else (8 if rows <= 8 else 16 if rows <= 16 else 32, 4)
+    """Into how many ranges of pages ``tree_attention`` cuts a request's cells: as many as fill the SMs with its blocks, two pages at least each; up to 8 join in
+    one kernel, more cost a second one (4 us) and are taken for 128 pages and more, of eight pages each.  (32 heads on 8 of 128, e4m3, us: one request of 1,001
+    cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 52 in 8, 29 in 62; eight of 2,176 29, 17 in 6 to 8, 21 in
+    16; 16 of 4,001 60, 30 in 4, 37 in 8; 64 of up to 4,097 85, 84 in 2, 120 in 8; 128 of 2,001 97, 107 in 2.  With 64 drafted tokens, four requests of up to 8,256
+    175, 75 in 4, 90 in 8; one request of 32,064 842, 161 in 8, 102 in 16.)"""
+    height, per_sm = (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
-    return max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
+    n = max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
+    return n if n <= TREE_CLUSTER else TREE_CLUSTER if pages < 128 else max(TREE_CLUSTER, min(n, pages // 8))
 
 
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
@@ -3188,12 +3193,14 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: to
         raise KernelError(f"{who}: {top} alternatives (0 to min(vocabulary {v}, {LOGPROBS_TOP}))")
     # all results in one allocation, each kind in one run: log p, rank, entropy, then ids and log p of the best
     flat = torch.empty(n * (3 + 2 * top), dtype=torch.float32, device=logits.device)
-    at, ints = flat.data_ptr(), flat.view(torch.int32)
+    at = flat.data_ptr()
     fn = _fn("logprobs", "lgml_token_logprobs", [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                  c_void_p])
     _check("logprobs", fn(logits.data_ptr(), max(ld, v), n, v, ids.data_ptr(), int(top), _logprob_slices(n, v), at, at + 4 * n, at + 8 * n, at + 12 * n,
                           at + 12 * n + 4 * n * top, status.data_ptr(), _stream()), who)
-    return TokenLogprobs(flat[:n], ints[n:2 * n], flat[2 * n:3 * n], ints[3 * n:3 * n + n * top].view(n, top), flat[3 * n + n * top:3 * n + 2 * n * top].view(n, top))
+    ints, many = flat.view(torch.int32), (n, top)
+    return TokenLogprobs(flat.as_strided((n,), (1,), 0), ints.as_strided((n,), (1,), n), flat.as_strided((n,), (1,), 2 * n),
+                         ints.as_strided(many, (top, 1), 3 * n), flat.as_strided(many, (top, 1), 3 * n + n * top))
 
 
 @functools.lru_cache(maxsize=None)
