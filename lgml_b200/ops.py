@@ -3087,7 +3087,7 @@ def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int
     cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 52 in 8, 29 in 62; eight of 2,176 29, 17 in 6 to 8, 21 in
     16; 16 of 4,001 60, 30 in 4, 37 in 8; 64 of up to 4,097 85, 84 in 2, 120 in 8; 128 of 2,001 97, 107 in 2.  With 64 drafted tokens, four requests of up to 8,256
     175, 75 in 4, 90 in 8; one request of 32,064 842, 161 in 8, 102 in 16.)"""
-    height, per_sm = (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
+    height, per_sm = (256, 1) if tall and rows > 128 else (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
     n = max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
@@ -3126,7 +3126,8 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         if visible.numel() != n:
             raise KernelError(f"{who}: one mask a token")
     rows = max_new_tokens * (n_heads // hkv)
-    tall = rows >= TREE_TALL_ROWS and d in (64, 128) and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
+    # (the tcgen05 kernel takes a row's maximum before it scales)
+    tall = rows >= TREE_TALL_ROWS and d in (64, 128) and scale > 1e-6 and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
     if n_splits is None:
         n_splits = tree_splits(seqs, hkv, rows, max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page), page, tall)
     if n_splits > TREE_CLUSTER:
