@@ -1,5 +1,5 @@
 // Attention of the new tokens of a request over its paged cache (attention_tree.cu has the definition) where a KV head has many rows: tokens x heads
-// of 33 and more.  There the products are what takes time, so they are on tcgen05, one tile of 128 rows a block, or two where there are more rows:
+// of 17 or 33 and more.  There the products are what takes time, so they are on tcgen05, one tile of 128 rows a block, or two where there are more rows:
 //     S[128, 64] = Q[128, D] . K_page^T        O[128, D] += P[128, 64] . V_page        accumulators in tensor memory
 // A thread a row does the softmax and writes P back into tensor memory, over the scores it came from; groups of two warps bring pages' keys and values into
 // stages of shared memory, which the tiles share; a warp a tile issues its products.  A tile has two buffers of scores: those of page it + 2 are issued behind the
@@ -22,8 +22,11 @@
 // rows of a page, and a page of two tiles takes 2,200 (the tensor cores are at work for 512 of them).  Two tiles a block convert a page once for 256 rows.
 // Three groups bring pages to two tiles, since sixteen warps are as many as leave a thread 128 registers.  Measured, four requests of up to 8,256 cells, 64
 // drafted tokens, 32 heads on 8 of 128, e4m3: 50 us (one tile a block, two threads a row, columns scaled one by one: 75; conversions by integer
-// arithmetic instead of the conversion instruction: 50; four groups at 96 registers: 59); 27 drafted tokens of one request over 2,203 cells, bfloat16: 15.5.
+// arithmetic instead of the conversion instruction: 50; four groups at 96 registers: 59); 27 drafted tokens of one request over 2,203 cells, bfloat16: 15.6.
 // Of those 50: 2 until the queries are in, 36 for 25 pages, 4 to join the ranges; the rest is blocks that start after others.
+// Two tiles a block from 129 rows on, and a block an SM, against one tile and two blocks (us, each at its best cut; 2,064 cells, eight requests): 256 rows e4m3 38 / 58,
+// bfloat16 36 / 44, heads of 64 27 / 29; 132 rows e4m3 35 / 53, bfloat16 31 / 40; one request of 256 rows bfloat16 20 / 18; 512 rows, two of 8,256 cells: e4m3 61 / 89,
+// bfloat16 51 / 67.
 // Waits on mbarriers are bounded (status 14).
 #include "tree_common.cuh"
 

@@ -10,7 +10,11 @@
 // written again keeps its codes.  The exponent is kept as a byte, e + 127, in an array of its own: 1 byte on 128.
 //
 // Cells and positions differ for drafted tokens that stand side by side at one position: the cell is where a token's key
-// lies (table[cell / 64], cell % 64), the position what it is turned by.
+// lies (table[cell / 64], cell % 64), the position what it is turned by.  The cells of a call differ (two tokens in one cell leave either's entries there).
+//
+// Both directions are memory's: every entry is read and written once.  What they take (32 heads on 8 of 128, launches back to back): one token e4m3 1.4 us,
+// 8 tokens 1.5, 2,048 tokens 10.2 (46 MB, 4.6 TB/s) in e4m3 and 9.1 (50 MB, 5.5 TB/s) in bfloat16; reading 1,531 pages back 98 us (604 MB, 6.2 TB/s, 0.94 of the
+// measured copy rate), 34 pages 5.4.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -144,7 +148,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
 // The same for many tokens, bfloat16 in, heads of 64 or 128 entries that turn whole: a block a token, whose angles are computed once for all its
 // heads; sixteen lanes a head, each with P = D / 32 neighbouring entries of the first half of the head and P of the second ("half"), or 2 P
 // neighbouring entries ("adjacent"): either way the pairs that turn together are in one thread, and loads and stores are 4 P and 2 P bytes wide.
-constexpr int WIDE_THREADS = 256, WIDE_FROM = 24;
+// A thread's first loads set out ahead of the trip to the block table.  (us this way and by a warp a head, heads of 128: 64 tokens e4m3 2.5 / 2.3, bfloat16
+// 1.9 / 2.0; 128 tokens 2.5 / 3.7 and 2.3 / 3.5; 2,048 tokens 10 / 39 and 9 / 37.  Two heads on their way instead of three: 13.5 at 2,048; four: 12.9.)
+constexpr int WIDE_THREADS = 256, WIDE_FROM = 65, WIDE_HEADS = 3;      // (heads a thread has on their way)
 template <int P> struct Vec;
 template <> struct Vec<2> { using type = unsigned; };
 template <> struct Vec<4> { using type = uint2; };
@@ -161,30 +167,35 @@ __global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
     __shared__ float2 turn[D / 2];           // (cos, sin) of pair i
     const int t = blockIdx.x, tid = threadIdx.x, l = tid & 15;
     const int pos = early_int(positions + t), cell = cells ? early_int(cells + t) : pos, seq = early_int(seq_of_token + t), blk = cell / PAGE;
-    const int page = cell >= 0 && blk < max_blocks && seq >= 0 && seq < n_seqs ? early_int(block_table + (size_t)seq * max_blocks + blk) : -1;
     if (tid < D / 2) {
         float sn, cs;
         rope_sincos(pos, early_weight(inv_freq + tid), inv_freq_lo ? early_weight(inv_freq_lo + tid) : 0.f, &sn, &cs);
         turn[tid] = make_float2(cs, sn);
     }
-    const bool there = page >= 0 && page < n_pages;
-    if (!there && n_heads > H && tid == 0) atomicExch(status, 2);      // the host reserves pages first; never write outside the pool
-    __syncthreads();
     pdl_wait();
     // entries e of the first run and of the second; pair i of the thread is (x[i], x[P + i]) or, adjacent, (x[2 i], x[2 i + 1])
     const int run0 = ADJACENT ? 2 * P * l : P * l, run1 = ADJACENT ? run0 + P : run0 + D / 2;
     constexpr int UNITS = WIDE_THREADS / 16;
-    for (int base = 0; base < n_heads; base += 2 * UNITS) {       // (both heads of a warp go round as often)
+    bool there = false;
+    int page = -1;
+    for (int base = 0; base < n_heads; base += WIDE_HEADS * UNITS) {       // (both heads of a warp go round as often)
         const int head = base + tid / 16;
-        Half raw[2][2];
+        Half raw[WIDE_HEADS][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < WIDE_HEADS; ++k)
             if (head + k * UNITS < n_heads) {
                 const __nv_bfloat16 *p = src + (size_t)t * lds + (size_t)(head + k * UNITS) * D;
                 raw[k][0] = __ldcg(reinterpret_cast<const Half *>(p + run0)), raw[k][1] = __ldcg(reinterpret_cast<const Half *>(p + run1));
             }
+        if (base == 0) {
+            // (behind the first loads: a trip to the table and the other threads' angles)
+            page = cell >= 0 && blk < max_blocks && seq >= 0 && seq < n_seqs ? early_int(block_table + (size_t)seq * max_blocks + blk) : -1;
+            there = page >= 0 && page < n_pages;
+            if (!there && n_heads > H && tid == 0) atomicExch(status, 2);      // the host reserves pages first; never write outside the pool
+            __syncthreads();
+        }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < WIDE_HEADS; ++k) {
             const int h = head + k * UNITS;
             const bool mine = h < n_heads;              // (the lanes of a head are together in this, and in the reduction below)
             float x[2 * P];
@@ -200,7 +211,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
                 }
             }
             const size_t vec = there ? ((size_t)page * Hkv + (h < H + Hkv ? h - H : h - H - Hkv)) * PAGE + cell % PAGE : 0;
-            if (Q8) {
+            if (Q8 && (h | 1) >= H) {              // (one of the warp's two heads is a key or a value)
                 float amax = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * P; ++i) amax = fmaxf(amax, finite_abs(x[i]));
@@ -238,7 +249,8 @@ __global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
 }
 
 // Page list[i] of the pool as bfloat16 page i of the output: a block per (page, KV head, keys or values), 16 codes a thread and turn.
-// An entry below zero leaves its page of the output as it is; one past the pool does too, and sets the status.
+// An entry below zero leaves its page of the output as it is; one past the pool does too, and sets the status.  (Nothing is used twice: what counts is that
+// every thread's four or eight loads are 16 bytes wide and on their way together.)
 constexpr int READ_THREADS = 128;
 __global__ void __launch_bounds__(READ_THREADS) kv_read_kernel(const uint8_t *__restrict__ k_pages, const uint8_t *__restrict__ v_pages,
                                                                const uint8_t *__restrict__ k_exps, const uint8_t *__restrict__ v_exps, int n_pages,

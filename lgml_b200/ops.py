@@ -2932,7 +2932,10 @@ def paged_attention(q, batch, cache, out, n_heads: int, scale: float, window: in
 E4M3 = torch.float8_e4m3fn
 TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
 TREE_MAX_DIM = 128
-TREE_TALL_ROWS = 33         # rows of a KV head (tokens x heads) from which it takes 128 of them a block, on tcgen05
+# Rows of a KV head (tokens x heads) from which ``tree_attention`` takes 128 or 256 of them a block, on tcgen05; the second number where there are more e4m3
+# pages' KV heads than SMs (us there and on mma.sync, 32 heads on 8 of 128, 2,000 cells; 16 rows: one request 14 / 13, eight 31 / 21; 20 rows: bfloat16, one 13 / 18,
+# eight 26 / 35, 64 148 / 173; e4m3 15 / 18, 31 / 31, 174 / 146; 32 rows: e4m3 15 / 20, 31 / 36, 177 / 154; 36 rows: 15 / 24, 31 / 52).
+TREE_TALL_ROWS = (17, 33)
 TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
 
@@ -3086,7 +3089,7 @@ def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int
     one kernel, more cost a second one (4 us) and are taken for 128 pages and more, of eight pages each.  (32 heads on 8 of 128, e4m3, us: one request of 1,001
     cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 52 in 8, 29 in 62; eight of 2,176 29, 17 in 6 to 8, 21 in
     16; 16 of 4,001 60, 30 in 4, 37 in 8; 64 of up to 4,097 85, 84 in 2, 120 in 8; 128 of 2,001 97, 107 in 2.  With 64 drafted tokens, four requests of up to 8,256
-    175, 75 in 4, 90 in 8; one request of 32,064 842, 161 in 8, 102 in 16.)"""
+    155, 84 in 2, 50 in 4, 88 in 8; 36 rows of eight requests of 2,009 73, 42 in 2, 31 in 4, 43 in 8.)"""
     height, per_sm = (256, 1) if tall and rows > 128 else (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
@@ -3127,7 +3130,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
             raise KernelError(f"{who}: one mask a token")
     rows = max_new_tokens * (n_heads // hkv)
     # (the tcgen05 kernel takes a row's maximum before it scales)
-    tall = rows >= TREE_TALL_ROWS and d in (64, 128) and scale > 1e-6 and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
+    tall = rows >= TREE_TALL_ROWS[k_exps is not None and seqs * hkv > sm_count()] and d in (64, 128) and scale > 1e-6 and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
     if n_splits is None:
         n_splits = tree_splits(seqs, hkv, rows, max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page), page, tall)
     if n_splits > TREE_CLUSTER:

@@ -428,6 +428,13 @@ def test_attention_of_tiles_of_many_rows(H, G, D, eight):
 
 
 @pytest.mark.parametrize("eight", [True, False])
+def test_attention_of_many_requests_with_a_few_drafted_tokens(eight):
+    p = Problem([5, 8, 3] * 25, [70, 0, 64] * 25, 8, 2, 64, eight, tree=True, seed=4)
+    for n_splits in (None, 2):
+        p.check(p.run(n_splits=n_splits))
+
+
+@pytest.mark.parametrize("eight", [True, False])
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-7, 2.0])
 def test_attention_with_any_scale(scale, eight):
     for lens in ([1, 3], [12, 40]):
