@@ -5,16 +5,16 @@
 //     e = clamp(ceil(log2(amax / 448)), -60, 119)     amax over the vector's finite entries; all zero: -60
 //     code_i = e4m3(x_i 2^-e), to nearest;  NaN and infinities: NaN
 // so the largest entry lands in (224, 448], and x 2^-e and code 2^e are exact in float32 and, the second, in bfloat16: a
-// vector is rounded once, when it is written, from the float32 result of the rotation (half a step of four bits,
-// 2^-4 of an entry's size, or 2^-10 2^e for entries under 2^-6 2^e).  Reading back rounds nothing, and a vector that is read back and
+// vector is rounded once, when it is written (half a step of four bits, 2^-4 of an entry's size, or 2^-10 2^e for entries under 2^-6 2^e).  A key that is to
+// be codes is turned in float64: float32's last bit would put one entry in 3 10^5 on the other side of a border between codes.  Reading back rounds nothing, and a vector that is read back and
 // written again keeps its codes.  The exponent is kept as a byte, e + 127, in an array of its own: 1 byte on 128.
 //
 // Cells and positions differ for drafted tokens that stand side by side at one position: the cell is where a token's key
 // lies (table[cell / 64], cell % 64), the position what it is turned by.  The cells of a call differ (two tokens in one cell leave either's entries there).
 //
-// Both directions are memory's: every entry is read and written once.  What they take (32 heads on 8 of 128, launches back to back): one token e4m3 1.4 us,
-// 8 tokens 1.5, 2,048 tokens 10.2 (46 MB, 4.6 TB/s) in e4m3 and 9.1 (50 MB, 5.5 TB/s) in bfloat16; reading 1,531 pages back 98 us (604 MB, 6.2 TB/s, 0.94 of the
-// measured copy rate), 34 pages 5.4.
+// Both directions are memory's: every entry is read and written once.  What they take (32 heads on 8 of 128, launches back to back): one token e4m3 1.5 us,
+// 8 tokens 1.6, 2,048 tokens 12.4 (46 MB, 3.7 TB/s; 10.2 with the rotation in float32) in e4m3 and 9.1 (50 MB, 5.5 TB/s) in bfloat16; reading 1,531 pages back
+// 98 us (604 MB, 6.2 TB/s, 0.94 of the measured copy rate), 34 pages 5.4.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -45,6 +45,12 @@ __device__ __forceinline__ unsigned short e4m3_pair(float a, float b, float inv)
     return r;
 }
 
+// The sine and cosine of pos (f + f_lo), in float64.
+__device__ __forceinline__ void sincos_64(int pos, float f, float f_lo, double *s, double *c) {
+    const double a = (double)pos * ((double)f + (double)f_lo), k = rint(a * 0.15915494309189535);
+    sincos(fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586, a)), s, c);            // (2 pi in two parts)
+}
+
 // Few tokens, and any head size: a warp a head of a token; a lane holds pairs lane, lane + 32, .. (PAIRS at most) of the head, so the vector's
 // largest entry is one warp reduction.  pairing and the treatment of entries past n_rot as in rope_cache.cu.
 template <typename TS, bool Q8, int PAIRS>
@@ -72,7 +78,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
     float a[PAIRS], b[PAIRS];
     int d0[PAIRS], d1[PAIRS];
     float sn[PAIRS], cs[PAIRS];
-    const bool turns = head < H + Hkv;
+    double sn64[Q8 ? PAIRS : 1], cs64[Q8 ? PAIRS : 1];
+    const bool turns = head < H + Hkv, coded = Q8 && head >= H;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
         const int j = lane + 32 * i;
@@ -81,7 +88,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
         if (turns && j < half_rot) {
             d0[i] = pairing ? 2 * j : j;
             d1[i] = pairing ? 2 * j + 1 : j + half_rot;
-            rope_sincos(pos, early_weight(inv_freq + j), inv_freq_lo ? early_weight(inv_freq_lo + j) : 0.f, &sn[i], &cs[i]);
+            const float f = early_weight(inv_freq + j), f_lo = inv_freq_lo ? early_weight(inv_freq_lo + j) : 0.f;
+            if (coded) sincos_64(pos, f, f_lo, &sn64[Q8 ? i : 0], &cs64[Q8 ? i : 0]);
+            else rope_sincos(pos, f, f_lo, &sn[i], &cs[i]);
         } else {
             d0[i] = 2 * j;
             d1[i] = d0[i] + 1;
@@ -108,8 +117,13 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
         if (j >= half_d) continue;
         if (bias) a[i] += bias[col + d0[i]], b[i] += bias[col + d1[i]];
         if (turns && j < half_rot) {
-            const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
-            a[i] = x, b[i] = y;
+            if (coded) {
+                const double x = a[i], y = b[i], sn_i = sn64[Q8 ? i : 0], cs_i = cs64[Q8 ? i : 0];
+                a[i] = (float)(x * cs_i - y * sn_i), b[i] = (float)(x * sn_i + y * cs_i);
+            } else {
+                const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
+                a[i] = x, b[i] = y;
+            }
         }
         if (Q8) amax = fmaxf(amax, fmaxf(finite_abs(a[i]), finite_abs(b[i])));
     }
@@ -149,7 +163,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
 // heads; sixteen lanes a head, each with P = D / 32 neighbouring entries of the first half of the head and P of the second ("half"), or 2 P
 // neighbouring entries ("adjacent"): either way the pairs that turn together are in one thread, and loads and stores are 4 P and 2 P bytes wide.
 // A thread's first loads set out ahead of the trip to the block table.  (us this way and by a warp a head, heads of 128: 64 tokens e4m3 2.5 / 2.3, bfloat16
-// 1.9 / 2.0; 128 tokens 2.5 / 3.7 and 2.3 / 3.5; 2,048 tokens 10 / 39 and 9 / 37.  Two heads on their way instead of three: 13.5 at 2,048; four: 12.9.)
+// 1.9 / 2.0; 128 tokens 2.8 / 3.7 and 2.3 / 3.5; 2,048 tokens 12 / 39 and 9 / 37.  Two or four heads on their way instead of three: 2 and 1.5 us more at 2,048.
+// Six blocks an SM instead of the four that the registers leave: 12.2 at 2,048, 45 instead of 50 at 8,192, but 5.3 instead of 3.8 at 512.)
 constexpr int WIDE_THREADS = 256, WIDE_FROM = 65, WIDE_HEADS = 3;      // (heads a thread has on their way)
 template <int P> struct Vec;
 template <> struct Vec<2> { using type = unsigned; };
@@ -165,11 +180,20 @@ __global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
     constexpr int D = 32 * P;
     using Half = typename Vec<P>::type;
     __shared__ float2 turn[D / 2];           // (cos, sin) of pair i
+    __shared__ double2 turn64[Q8 ? D / 2 : 1];
     const int t = blockIdx.x, tid = threadIdx.x, l = tid & 15;
     const int pos = early_int(positions + t), cell = cells ? early_int(cells + t) : pos, seq = early_int(seq_of_token + t), blk = cell / PAGE;
     if (tid < D / 2) {
         float sn, cs;
-        rope_sincos(pos, early_weight(inv_freq + tid), inv_freq_lo ? early_weight(inv_freq_lo + tid) : 0.f, &sn, &cs);
+        const float f = early_weight(inv_freq + tid), f_lo = inv_freq_lo ? early_weight(inv_freq_lo + tid) : 0.f;
+        if (Q8) {
+            double sn64, cs64;
+            sincos_64(pos, f, f_lo, &sn64, &cs64);
+            turn64[tid] = make_double2(cs64, sn64);
+            sn = (float)sn64, cs = (float)cs64;
+        } else {
+            rope_sincos(pos, f, f_lo, &sn, &cs);
+        }
         turn[tid] = make_float2(cs, sn);
     }
     pdl_wait();
@@ -201,7 +225,15 @@ __global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
             float x[2 * P];
 #pragma unroll
             for (int i = 0; i < 2 * P; ++i) x[i] = mine ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(raw[k])[i]) : 0.f;
-            if (h < H + Hkv) {
+            if (Q8 && h >= H && h < H + Hkv) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int a = ADJACENT ? 2 * i : i, b = ADJACENT ? 2 * i + 1 : P + i;
+                    const double2 f = turn64[Q8 ? P * l + i : 0];
+                    const double u = x[a], v = x[b];
+                    x[a] = (float)(u * f.x - v * f.y), x[b] = (float)(u * f.y + v * f.x);
+                }
+            } else if (h < H + Hkv) {
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const int a = ADJACENT ? 2 * i : i, b = ADJACENT ? 2 * i + 1 : P + i;

@@ -3004,7 +3004,8 @@ def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, bloc
     codes and one power of two, e = clamp(ceil(log2(amax / 448)), -60, 119) over its finite entries, kept as e + 127; an entry is
     rounded once, from float32, to half a step of four bits; NaN and infinities become NaN.  Without them the pages are bfloat16.
     ``qkv``: bfloat16 [tokens, (H + 2 Hkv) D], or ``Partials``; q comes out in bfloat16, in ``q_out`` (never in place; made if None).
-    ``inv_freq``, ``n_rot``, ``pairing`` as for ``rope_kv_write``."""
+    ``inv_freq``, ``n_rot``, ``pairing`` as for ``rope_kv_write``.  The tokens of a call have cells of their own each.  Positions, cells, ``seq_of_token`` and
+    the block table are a step's description, which is complete before the kernels ahead are launched, as everywhere here (they are read ahead)."""
     who = "rope_kv_store"
     dev = _device_of(who, k_pages, "key pages")
     n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)
@@ -3108,7 +3109,9 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     included, if it is to see itself); None: a chain, every token sees those up to itself.  Old cells are all seen; with ``window`` > 0 only
     cells whose position is above the token's position - window (an old cell's position is its number).  A row that sees nothing is zeros.
     Requests that bring more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
-    included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read."""
+    included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read.  Positions, first rows, counts, masks and the
+    block table are a step's description, which is complete before the kernels ahead are launched.  Results depend on the number of ranges and on the kernel
+    that the rows take in their rounding only; one call's are the same each time."""
     who = "tree_attention"
     dev = _device_of(who, k_pages, "key pages")
     n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)

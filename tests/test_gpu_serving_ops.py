@@ -138,6 +138,28 @@ def test_store_writes_cells_and_turns_by_positions(H, G, D, n_rot, pairing, part
         assert torch.equal(raw(pool)[~written], raw(old)[~written])
 
 
+@pytest.mark.parametrize("N,D,pairing", [(40, 128, "half"), (40, 96, "adjacent"), (500, 128, "half"), (500, 64, "adjacent")])
+def test_keys_in_codes_are_those_of_the_rotation_in_64_bits(N, D, pairing):
+    """Both kernels; positions up to 500,000.  (float32's sine alone, off by 2^-25, would put about one code in 10^5 on the other side of a border.)"""
+    from lgml_b200 import ops
+
+    H, G = 2, 8
+    g = torch.Generator().manual_seed(N + D)
+    qkv = torch.randn(N, (H + 2 * G) * D, generator=g).to(torch.bfloat16)
+    positions = [(i * 997) % 500000 for i in range(N)]
+    table, pages = tables([N])
+    exact, freq = frequencies(D)
+    k, v, ke, ve = poison(pages, G, D, True)
+    st = status()
+    ops.rope_kv_store(qkv.to(DEV), ints(positions), ints([0] * N), ints(table), freq, D, pairing, k, v, H, G, D, st, cells=ints(range(N)), k_exps=ke, v_exps=ve)
+    assert st.item() == 0
+    page, at = torch.tensor([table[0][c // PAGE] for c in range(N)]), torch.arange(N) % PAGE
+    x = turned(qkv.double().view(N, H + 2 * G, D)[:, H:H + G], positions, freq.double().sum(0).cpu(), D, pairing).float()
+    e = exponent(x.double())
+    assert torch.equal(ke.cpu()[page, :, at].int(), (e + 127).int())
+    assert torch.equal(k.view(torch.uint8).cpu()[page, :, at], torch.ldexp(x, -e[..., None]).to(E4M3).view(torch.uint8))
+
+
 def test_store_of_special_vectors_and_back():
     """Zeros, the largest and the smallest numbers, NaN and infinities; a vector read back and written again keeps its codes."""
     from lgml_b200 import ops
