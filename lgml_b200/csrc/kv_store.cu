@@ -6,7 +6,7 @@
 //     code_i = e4m3(x_i 2^-e), to nearest;  NaN and infinities: NaN
 // so the largest entry lands in (224, 448], and x 2^-e and code 2^e are exact in float32 and, the second, in bfloat16: a
 // vector is rounded once, when it is written (half a step of four bits, 2^-4 of an entry's size, or 2^-10 2^e for entries under 2^-6 2^e).  A key that is to
-// be codes is turned in float64: float32's last bit would put one entry in 3 10^5 on the other side of a border between codes.  Reading back rounds nothing, and a vector that is read back and
+// be codes is turned in float64: float32's last bit would put a few of 10^6 entries on the other side of a border between codes.  Reading back rounds nothing, and a vector that is read back and
 // written again keeps its codes.  The exponent is kept as a byte, e + 127, in an array of its own: 1 byte on 128.
 //
 // Cells and positions differ for drafted tokens that stand side by side at one position: the cell is where a token's key

@@ -2938,6 +2938,12 @@ TREE_MAX_DIM = 128
 TREE_TALL_ROWS = (17, 33)
 TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
+_STORE_ARGS = [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+               c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+_READ_ARGS = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]
+_LOGPROBS_ARGS = [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+_TREE_ARGS = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+              c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p]
 
 
 def _are(who: str, dev: int, dtype: torch.dtype, ndim: int, names: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -2976,7 +2982,8 @@ def _kv_pages(who: str, dev: int, k_pages, v_pages, k_exps, v_exps) -> tuple:
         raise KernelError(f"{who}: key and value pages must be of one shape ({tuple(shape)}, {tuple(v_pages.shape)})")
     if k_exps is not None:
         _are(who, dev, torch.uint8, 3, "key exponents, value exponents", k_exps, v_exps)
-        if k_exps.shape != shape[:3] or v_exps.shape != shape[:3]:
+        vectors = shape[:3]
+        if k_exps.shape != vectors or v_exps.shape != vectors:
             raise KernelError(f"{who}: exponents are [pages, KV heads, page], not {tuple(k_exps.shape)} and {tuple(v_exps.shape)}")
     return shape
 
@@ -3049,9 +3056,7 @@ def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, bloc
     if n_rot % 2 or n_rot < 0 or n_rot > head_dim or n_freq < n_rot // 2:
         raise KernelError(f"{who}: n_rot {n_rot} must be even, at most head_dim, and have n_rot / 2 frequencies")
     seqs, blocks = block_table.shape
-    fn = _fn("kv_store", "lgml_rope_kv_store", [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                                c_int, c_int, c_int, c_void_p, c_void_p])
+    fn = _fn("kv_store", "lgml_rope_kv_store", _STORE_ARGS)
     _check("kv_store", fn(src.data_ptr(), src_type, lds, n_parts, stride, _ptr(bias), q_out.data_ptr(), ldq, positions.data_ptr(), _ptr(cells),
                           seq_of_token.data_ptr(), block_table.data_ptr(), seqs, blocks, inv_freq.data_ptr(), low, n_rot, PAIRING[pairing],
                           k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, n, n_heads, n_kv_heads, head_dim,
@@ -3079,7 +3084,7 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
     if k_out.shape != shape or v_out.shape != shape or status.numel() != 1:
         raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}, and the status is one int32")
-    fn = _fn("kv_store", "lgml_kv_read", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
+    fn = _fn("kv_store", "lgml_kv_read", _READ_ARGS)
     _check("kv_store", fn(k_pages.data_ptr(), v_pages.data_ptr(), k_exps.data_ptr(), v_exps.data_ptr(), n_pages, page, pages.data_ptr(), n, k_out.data_ptr(),
                           v_out.data_ptr(), hkv, d, status.data_ptr(), _stream()), who)
     return k_out, v_out
@@ -3144,8 +3149,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         if scratch.numel() < need:
             raise KernelError(f"{who}: scratch of {scratch.numel()} floats, {need} needed")
     lib, name = ("attention_tree_tall", "lgml_tree_attention_tall") if tall else ("attention_tree", "lgml_tree_attention")
-    fn = _fn(lib, name, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
-                         c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+    fn = _fn(lib, name, _TREE_ARGS)
     _check(lib, fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
                    blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
                    scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
@@ -3201,8 +3205,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: to
     # all results in one allocation, each kind in one run: log p, rank, entropy, then ids and log p of the best
     flat = torch.empty(n * (3 + 2 * top), dtype=torch.float32, device=logits.device)
     at = flat.data_ptr()
-    fn = _fn("logprobs", "lgml_token_logprobs", [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                 c_void_p])
+    fn = _fn("logprobs", "lgml_token_logprobs", _LOGPROBS_ARGS)
     _check("logprobs", fn(logits.data_ptr(), max(ld, v), n, v, ids.data_ptr(), int(top), _logprob_slices(n, v), at, at + 4 * n, at + 8 * n, at + 12 * n,
                           at + 12 * n + 4 * n * top, status.data_ptr(), _stream()), who)
     ints, many = flat.view(torch.int32), (n, top)

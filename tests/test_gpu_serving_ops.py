@@ -140,7 +140,7 @@ def test_store_writes_cells_and_turns_by_positions(H, G, D, n_rot, pairing, part
 
 @pytest.mark.parametrize("N,D,pairing", [(40, 128, "half"), (40, 96, "adjacent"), (500, 128, "half"), (500, 64, "adjacent")])
 def test_keys_in_codes_are_those_of_the_rotation_in_64_bits(N, D, pairing):
-    """Both kernels; positions up to 500,000.  (float32's sine alone, off by 2^-25, would put about one code in 10^5 on the other side of a border.)"""
+    """Both kernels; positions up to 500,000.  (float32's sine alone would put a few of 10^6 codes on the other side of a border.)"""
     from lgml_b200 import ops
 
     H, G = 2, 8
