@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
     const __nv_bfloat16 *__restrict__ q, int ldq, const int *__restrict__ positions, const int *__restrict__ seq_start, const int *__restrict__ seq_pos0,
     const long long *__restrict__ visible, const int *__restrict__ block_table, int max_blocks, const uint8_t *__restrict__ k_pages,
     const uint8_t *__restrict__ v_pages, const uint8_t *__restrict__ k_exps, const uint8_t *__restrict__ v_exps, int n_pages, __nv_bfloat16 *__restrict__ out,
-    int ldo, float *__restrict__ part_o, float2 *__restrict__ part_ml, int n_splits, int clustered, int n_tokens, int H, int Hkv, int n_chunks, int limit,
+    int ldo, float *__restrict__ part_o, float2 *__restrict__ part_ml, int n_splits, int clustered, int n_tokens, int H, int Hkv, int n_chunks, int least, int limit,
     float scale, int window, int *__restrict__ status) {
     constexpr int KB = D / 64;                        // 64-element blocks along the head
     constexpr float P_UP = Q8 ? 7.f : 0.f;            // probabilities times 2^this, in the products and the sums: at most 2^15, float16 has numbers down to 2^-24
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
     const int s = blockIdx.x / n_splits, split = blockIdx.x - s * n_splits, kvh = blockIdx.y / n_chunks, chunk = blockIdx.y - kvh * n_chunks;
     const int row0 = early_int(seq_start + s), n = early_int(seq_start + s + 1) - row0, pos0 = early_int(seq_pos0 + s);
     const int group = H / Hkv, n_rows = n * group, r0 = chunk * ALL_ROWS;
-    if (n <= 0 || n > limit || r0 >= n_rows) return;
+    if (n < least || n > limit || r0 >= n_rows) return;
     if (row0 < 0 || row0 + n > n_tokens || pos0 < 0) {
         if (tid == 0) atomicExch(status, 3);
         return;
@@ -828,13 +828,13 @@ int launch_tiles(int D, bool q8, Args... args) {
 // As lgml_tree_attention, for head sizes of 64 and 128 and rows of q and out on 16 bytes.
 LGML_API int lgml_tree_attention_tall(const void *q, int ldq, const int *positions, const int *seq_start, const int *seq_pos0, const long long *visible,
                                       const int *block_table, int n_seqs, int max_blocks, const void *k_pages, const void *v_pages, const void *k_exps,
-                                      const void *v_exps, int n_pages, int page_size, void *out, int ldo, float *scratch, int n_splits, int n_tokens, int limit,
+                                      const void *v_exps, int n_pages, int page_size, void *out, int ldo, float *scratch, int n_splits, int n_tokens, int least, int limit,
                                       int H, int Hkv, int D, float scale, int window, int *status, cudaStream_t stream) {
     LGML_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && H > 0 && Hkv > 0 && max_blocks > 0 && n_pages >= 0, "tree_attention: bad sizes");
     LGML_REQUIRE(page_size == PAGE, "tree_attention: pages of %d tokens, this kernel takes %d", page_size, PAGE);
     LGML_REQUIRE(H % Hkv == 0, "tree_attention: %d heads are no multiple of %d KV heads", H, Hkv);
     LGML_REQUIRE(D == 64 || D == 128, "tree_attention: head_dim %d must be 64 or 128 here", D);
-    LGML_REQUIRE(limit >= 1 && limit <= MAX_NEW, "tree_attention: %d new tokens a request (1 to %d)", limit, MAX_NEW);
+    LGML_REQUIRE(least >= 1 && least <= limit && limit <= MAX_NEW, "tree_attention: %d to %d new tokens a request (1 to %d)", least, limit, MAX_NEW);
     LGML_REQUIRE(n_splits >= 1 && n_splits <= MAX_SPLITS, "tree_attention: %d key ranges (1 to %d)", n_splits, MAX_SPLITS);
     LGML_REQUIRE(n_splits <= MAX_CLUSTER || (scratch != nullptr && ((uintptr_t)scratch & 7) == 0), "tree_attention: several ranges need scratch memory");
     LGML_REQUIRE((k_exps == nullptr) == (v_exps == nullptr), "tree_attention: exponents for keys and values, or for neither");
@@ -851,9 +851,9 @@ LGML_API int lgml_tree_attention_tall(const void *q, int ldq, const int *positio
     float2 *part_ml = scratch ? reinterpret_cast<float2 *>(scratch + (size_t)n_tokens * H * n_splits * D) : nullptr;
 #define LGML_ARGS D, k_exps != nullptr, grid, clustered ? n_splits : 1, stream, (const __nv_bfloat16 *)q, ldq, positions, seq_start, seq_pos0, visible, block_table, \
                   max_blocks, (const uint8_t *)k_pages, (const uint8_t *)v_pages, (const uint8_t *)k_exps, (const uint8_t *)v_exps, n_pages,                     \
-                  (__nv_bfloat16 *)out, ldo, part_o, part_ml, n_splits, clustered, n_tokens, H, Hkv, n_chunks, limit, scale, window, status
+                  (__nv_bfloat16 *)out, ldo, part_o, part_ml, n_splits, clustered, n_tokens, H, Hkv, n_chunks, least, limit, scale, window, status
     const int rc = tiles == 2 ? launch_tiles<2>(LGML_ARGS) : launch_tiles<1>(LGML_ARGS);
 #undef LGML_ARGS
     if (rc || n_splits <= MAX_CLUSTER) return rc;
-    return tree_join(part_o, part_ml, seq_start, n_seqs, limit, n_tokens, out, ldo, n_splits, H, D, stream);
+    return tree_join(part_o, part_ml, seq_start, n_seqs, least, limit, n_tokens, out, ldo, n_splits, H, D, stream);
 }

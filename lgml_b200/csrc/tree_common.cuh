@@ -84,14 +84,14 @@ __device__ __forceinline__ void join_cluster(const float *merge, const float (*f
 // The ranges of one (token, head) in their order: a warp each.
 constexpr int JOIN_WARPS = 2;
 __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml,
-                                                                    const int *__restrict__ seq_start, int limit, int n_tokens, __nv_bfloat16 *__restrict__ out,
+                                                                    const int *__restrict__ seq_start, int least, int limit, int n_tokens, __nv_bfloat16 *__restrict__ out,
                                                                     int ldo, int n_splits, int H, int D) {
     pdl_trigger();
     pdl_wait();
     const int s = blockIdx.x / limit, j = blockIdx.x - s * limit, lane = threadIdx.x & 31;
     const int head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
     const int row0 = act_load(seq_start + s), n = act_load(seq_start + s + 1) - row0;
-    if (j >= n || n > limit || head >= H || row0 < 0 || row0 + n > n_tokens) return;
+    if (j >= n || n < least || n > limit || head >= H || row0 < 0 || row0 + n > n_tokens) return;
     const size_t at = ((size_t)(row0 + j) * H + head) * n_splits;
     // lane i has the maxima and sums of ranges i, i + 32, ..; eight ranges' outputs are under way at a time
     constexpr int PER_LANE = MAX_SPLITS / 32;
@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const float 
         if (d < D) store_row(out + (size_t)(row0 + j) * ldo + (size_t)head * D + d, o[u], l);
     }
 }
-int tree_join(const float *part_o, const float2 *part_ml, const int *seq_start, int n_seqs, int limit, int n_tokens, void *out, int ldo, int n_splits, int H, int D,
+int tree_join(const float *part_o, const float2 *part_ml, const int *seq_start, int n_seqs, int least, int limit, int n_tokens, void *out, int ldo, int n_splits, int H, int D,
               cudaStream_t stream) {
-    lgml_launch(tree_join_kernel, dim3(n_seqs * limit, (H + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, part_o, part_ml, seq_start, limit, n_tokens,
+    lgml_launch(tree_join_kernel, dim3(n_seqs * limit, (H + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, part_o, part_ml, seq_start, least, limit, n_tokens,
                 (__nv_bfloat16 *)out, ldo, n_splits, H, D);
     return lgml_launch_status("tree_attention_join");
 }

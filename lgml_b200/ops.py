@@ -2943,7 +2943,7 @@ _STORE_ARGS = [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_
 _READ_ARGS = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]
 _LOGPROBS_ARGS = [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
 _TREE_ARGS = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
-              c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p]
+              c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p]
 
 
 def _are(who: str, dev: int, dtype: torch.dtype, ndim: int, names: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -3106,14 +3106,14 @@ def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
                    v_pages: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, window: int, status: torch.Tensor, max_new_tokens: int,
                    max_kv_len: int, k_exps: Optional[torch.Tensor] = None, v_exps: Optional[torch.Tensor] = None, visible: Optional[torch.Tensor] = None,
-                   n_splits: Optional[int] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   n_splits: Optional[int] = None, scratch: Optional[torch.Tensor] = None, min_new_tokens: int = 1) -> torch.Tensor:
     """Attention of up to 64 new tokens a request over its cells, in bfloat16 pages or (with exponents) e4m3 ones.
 
     Request s brings rows ``seq_start[s]`` to ``seq_start[s + 1]`` of q; cells 0 to ``seq_pos0[s]`` - 1 are old, cell ``seq_pos0[s]`` + j is its j-th
     new token's.  ``visible`` (int64 [tokens], or None): bit j of a token's mask lets it see the request's j-th new token (its own bit
     included, if it is to see itself); None: a chain, every token sees those up to itself.  Old cells are all seen; with ``window`` > 0 only
     cells whose position is above the token's position - window (an old cell's position is its number).  A row that sees nothing is zeros.
-    Requests that bring more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
+    Requests that bring fewer than ``min_new_tokens`` or more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
     included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read.  Positions, first rows, counts, masks and the
     block table are a step's description, which is complete before the kernels ahead are launched.  Results depend on the number of ranges and on the kernel
     that the rows take in their rounding only; one call's are the same each time."""
@@ -3125,8 +3125,8 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     ldq = _rows_on(who, dev, q, "queries", torch.bfloat16, n_heads * d)
     n = q.shape[0]
     ldo = _rows_on(who, dev, out, "attention output", torch.bfloat16, n_heads * d, n)
-    if not 1 <= max_new_tokens <= TREE_TOKENS:
-        raise KernelError(f"{who}: {max_new_tokens} new tokens a request (1 to {TREE_TOKENS})")
+    if not 1 <= min_new_tokens <= max_new_tokens <= TREE_TOKENS:
+        raise KernelError(f"{who}: {min_new_tokens} to {max_new_tokens} new tokens a request (1 to {TREE_TOKENS})")
     _are(who, dev, torch.int32, 2, "block table", block_table)
     seqs, blocks = block_table.shape
     _are(who, dev, torch.int32, 1, "positions, first rows of requests, old cells of requests, status", positions, seq_start, seq_pos0, status)
@@ -3152,7 +3152,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     fn = _fn(lib, name, _TREE_ARGS)
     _check(lib, fn(q.data_ptr(), ldq, positions.data_ptr(), seq_start.data_ptr(), seq_pos0.data_ptr(), _ptr(visible), block_table.data_ptr(), seqs,
                    blocks, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exps), _ptr(v_exps), n_pages, page, out.data_ptr(), ldo,
-                   scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
+                   scratch.data_ptr() if n_splits > TREE_CLUSTER else 0, n_splits, n, int(min_new_tokens), int(max_new_tokens), n_heads, hkv, d, float(scale), int(window or 0),
                    status.data_ptr(), _stream()), who)
     return out
 
@@ -3163,9 +3163,19 @@ def cached_attention(q, batch, cache, out, n_heads: int, scale: float, window: i
     visible = getattr(batch, "visible", None)
     table, k, v = cache.block_table, cache.k, cache.v
     short = [n for n in batch.seq_lens if n <= TREE_TOKENS]
-    if short:
-        tree_attention(q, batch.positions, batch.seq_start, batch.seq_pos0, table, k, v, out, n_heads, scale, window, status, max_new_tokens=max(short),
-                       max_kv_len=batch.max_kv_len, k_exps=cache.k_exps, v_exps=cache.v_exps, visible=visible)
+    # Many requests of a token or a few beside one of many: each kind by the kernel that suits its rows (a block of 256 rows takes three times as long over a single
+    # token's four as one of eight does: 64 requests of up to 4,096 cells beside one of 64 new tokens 331 us in one call, 136 in two; 20 of them 154 and 64).
+    few = [n for n in short if n * (n_heads // k.shape[1]) < TREE_TALL_ROWS[0]]
+    parts = [(1, few), (max(few) + 1, [n for n in short if n > max(few)])] if few and len(few) < len(short) and len(few) * k.shape[1] > sm_count() else [(1, short)]
+    for least, lens in parts:
+        if not lens:
+            continue
+        splits = None
+        if len(parts) > 1:      # (ranges for the requests of this part)
+            rows, longest = max(lens) * (n_heads // k.shape[1]), batch.max_kv_len if not window else min(batch.max_kv_len, window + max(lens) + k.shape[2])
+            splits = tree_splits(len(lens), k.shape[1], rows, longest, k.shape[2], tall=rows >= TREE_TALL_ROWS[0] and k.shape[3] in (64, 128))
+        tree_attention(q, batch.positions, batch.seq_start, batch.seq_pos0, table, k, v, out, n_heads, scale, window, status, max_new_tokens=max(lens),
+                       max_kv_len=batch.max_kv_len, k_exps=cache.k_exps, v_exps=cache.v_exps, visible=visible, n_splits=splits, min_new_tokens=least)
     if len(short) == len(batch.seq_lens):
         return out
     if visible is not None:

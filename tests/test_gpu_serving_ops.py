@@ -417,6 +417,41 @@ def test_attention_leaves_longer_requests_and_the_space_between_rows_alone(eight
         p.check(wide[:, 4:4 + 512], skip=(1,))
 
 
+@pytest.mark.parametrize("eight", [True, False])
+@pytest.mark.parametrize("D", [64, 96])
+def test_attention_of_the_requests_between_two_lengths(D, eight):
+    """A call for the short requests and one for the longer ones are the call for all; each leaves the others' rows alone."""
+    lens = [1, 40, 2, 0, 64, 3]
+    p = Problem(lens, [100, 65, 0, 9, 130, 700], 8, 2, D, eight, tree=True, seed=2)
+    for n_splits in (1, 3, 10):
+        out = torch.full_like(p.q, 7.0)
+        p.run(most=3, n_splits=n_splits, out=out)
+        assert (out[1:41] == 7.0).all() and (out[43:107] == 7.0).all()
+        short = out.clone()
+        p.run(n_splits=n_splits, out=out, min_new_tokens=4)
+        for rows in (slice(0, 1), slice(41, 43), slice(107, 110)):
+            assert torch.equal(out[rows], short[rows])
+        p.check(out)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("D", [64, 32])
+def test_cached_attention_of_many_decoded_tokens_beside_short_portions(D, window):
+    from types import SimpleNamespace
+
+    from lgml_b200 import ops
+
+    lens, pos0 = [1] * 40 + [64] + [1] * 40 + [30, 1], [5 + 7 * i for i in range(40)] + [100] + [3 * i for i in range(40)] + [0, 1000]
+    p = Problem(lens, pos0, 8, 2, D, True, seed=6)
+    batch = SimpleNamespace(positions=ints(p.positions), seq_start=ints(p.start), seq_pos0=ints(pos0), seq_lens=lens, max_kv_len=1001, max_q_len=64)
+    cache = SimpleNamespace(block_table=ints(p.table), k=p.k, v=p.v, k_exps=p.ke, v_exps=p.ve)
+    st, out = status(), torch.empty_like(p.q)
+    before = ops.launch_count()
+    ops.cached_attention(p.q, batch, cache, out, p.H, p.scale, window, st)
+    assert ops.launch_count() - before == 2 and st.item() == 0
+    p.check(out, window=window)
+
+
 def test_attention_with_a_missing_page_sets_the_status():
     p = Problem([1, 1], [100, 10], 8, 2, 64, True)
     table = [row[:] for row in p.table]
