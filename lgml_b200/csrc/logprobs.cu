@@ -16,7 +16,7 @@
 // The slices of a row are a cluster, whose first block joins them, slice after slice, out of the others' shared memory.  All sums are float32.
 //
 // What bounds it is instructions (0.72 of the cycles issue one; maximum, exponential, two sums, the comparisons, a chunk's barriers and ranking), then memory:
-// 1,021 rows of 128,256 logits with 20 alternatives take 133 us (524 MB, 3.9 TB/s, 0.60 of the measured copy rate); 8 rows 12.5 us, a cluster of 16 blocks a row.
+// 1,021 rows of 128,256 logits with 20 alternatives take 130 us (524 MB, 4.0 TB/s, 0.61 of the measured copy rate; without alternatives 86, 0.93); 8 rows 12.5 us, a cluster of 16 blocks a row.
 // For those 1,021 rows: loads through registers and a ranking with every chunk 179; PER_SM blocks an SM: 2 224, 3 175, 4 133, 5 138, 6 190 (registers spill); two
 // stages 133; the list ranked with every entry that comes 132, from RANK_AT = 16 on 133, from 64 on 140 (what it saves is barriers where few entries come).
 #include <math.h>
@@ -259,18 +259,23 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const float *
         st.s += s2.x + s2.y;
         st.u += (u2.x + u2.y) * 0.6931471805599453f;
         if (largest >= x_id) {          // (mostly nobody: the given token is one of the best)
-            int above[2] = {0, 0};
-            bool equal = false;
+            // (an equal one counts if its index is lower: all of a chunk ahead of the id's, none of one behind it)
+            const int chunk_from = base - off;
+            float2 above = make_float2(0.f, 0.f);
+            if (chunk_from > id) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                above[j & 1] += x[j] > x_id ? 1 : 0;
-                equal |= x[j] == x_id;
-            }
-            greater += above[0] + above[1];
-            if (equal) {                // (the id itself, and a few)
+                for (int j = 0; j < PER; j += 2) above = add2(above, make_float2(x[j] > x_id ? 1.f : 0.f, x[j + 1] > x_id ? 1.f : 0.f));
+            } else if (chunk_from >= 0 && chunk_from + CHUNK <= id) {
 #pragma unroll
-                for (int j = 0; j < PER; ++j) greater += x[j] == x_id && first + (j >> 2) * THREADS * 4 + (j & 3) < id ? 1 : 0;
+                for (int j = 0; j < PER; j += 2) above = add2(above, make_float2(x[j] >= x_id ? 1.f : 0.f, x[j + 1] >= x_id ? 1.f : 0.f));
+            } else {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int i = first + (j >> 2) * THREADS * 4 + (j & 3);           // (below 0: -inf ahead of a row that starts off 16 bytes, which is no entry)
+                    above.x += x[j] > x_id || (x[j] == x_id && i >= 0 && i < id) ? 1.f : 0.f;
+                }
             }
+            greater += (int)(above.x + above.y);
         }
         // ---- the best ----
         auto collect = [&](int *count, auto pass) {

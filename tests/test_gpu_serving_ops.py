@@ -619,6 +619,23 @@ def test_logprobs_of_rows_that_are_hard(v):
         assert st.item() == 0
 
 
+def test_ranks_among_equal_logits_of_rows_off_16_bytes():
+    """Ids whose logit is -inf, or one of many equal ones, in rows that start at every place of 16 bytes: in the first chunk, a later one, the last."""
+    from lgml_b200 import ops
+
+    for v in (4, 4096, 9000):
+        for fill in (-math.inf, 0.0):
+            wide = torch.full((8, v + 1), fill)
+            wide[:, v // 2] = 1.0
+            x = wide.to(DEV)[:, 1:]                      # (v + 1 odd: rows start 1, 2, 3 .. places off)
+            for id in (0, 3, v - 2, v - 1):
+                st = status()
+                got = ops.token_logprobs(x, ints([id] * 8), 2, st)
+                row = wide[0, 1:]
+                want = int((row > row[id]).sum() + (row[:id] == row[id]).sum())
+                assert got.ranks.tolist() == [want] * 8 and st.item() == 0, (v, fill, id)
+
+
 def test_logprobs_without_an_id_and_with_one_outside():
     from lgml_b200 import ops
 
