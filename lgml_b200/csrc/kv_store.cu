@@ -13,7 +13,7 @@
 // lies (table[cell / 64], cell % 64), the position what it is turned by.  The cells of a call differ (two tokens in one cell leave either's entries there).
 //
 // Both directions are memory's: every entry is read and written once.  What they take (32 heads on 8 of 128, launches back to back): one token e4m3 1.5 us,
-// 8 tokens 1.6, 2,048 tokens 12.4 (46 MB, 3.7 TB/s; 10.2 with the rotation in float32) in e4m3 and 9.1 (50 MB, 5.5 TB/s) in bfloat16; reading 1,531 pages back
+// 8 tokens 1.6, 2,048 tokens 11.3 (46 MB, 4.1 TB/s; 10.2 with the rotation in float32) in e4m3 and 9.1 (50 MB, 5.5 TB/s) in bfloat16; reading 1,531 pages back
 // 98 us (604 MB, 6.2 TB/s, 0.94 of the measured copy rate), 34 pages 5.4.
 #include <cuda_fp16.h>
 #include <math.h>
@@ -163,15 +163,16 @@ __global__ void __launch_bounds__(WARPS * 32) kv_store_kernel(
 // heads; sixteen lanes a head, each with P = D / 32 neighbouring entries of the first half of the head and P of the second ("half"), or 2 P
 // neighbouring entries ("adjacent"): either way the pairs that turn together are in one thread, and loads and stores are 4 P and 2 P bytes wide.
 // A thread's first loads set out ahead of the trip to the block table.  (us this way and by a warp a head, heads of 128: 64 tokens e4m3 2.5 / 2.3, bfloat16
-// 1.9 / 2.0; 128 tokens 2.8 / 3.7 and 2.3 / 3.5; 2,048 tokens 12 / 39 and 9 / 37.  Two or four heads on their way instead of three: 2 and 1.5 us more at 2,048.
-// Six blocks an SM instead of the four that the registers leave: 12.2 at 2,048, 45 instead of 50 at 8,192, but 5.3 instead of 3.8 at 512.)
+// 1.9 / 2.0; 128 tokens 2.8 / 3.7 and 2.3 / 3.5; 2,048 tokens 11 / 39 and 9 / 37.  Two or four heads on their way instead of three: 2 and 1.5 us more at 2,048.
+// Heads of 128 in codes, five blocks an SM instead of the four that the registers would leave: 11.3 for 12.4 at 2,048, 46 for 50 at 8,192, 4.4 for 3.8 at 512;
+// six: 12.0, 44, 5.3.)
 constexpr int WIDE_THREADS = 256, WIDE_FROM = 65, WIDE_HEADS = 3;      // (heads a thread has on their way)
 template <int P> struct Vec;
 template <> struct Vec<2> { using type = unsigned; };
 template <> struct Vec<4> { using type = uint2; };
 template <> struct Vec<8> { using type = uint4; };
 template <int P, bool Q8, bool ADJACENT>
-__global__ void __launch_bounds__(WIDE_THREADS) kv_store_wide_kernel(
+__global__ void __launch_bounds__(WIDE_THREADS, Q8 && P == 4 ? 5 : 1) kv_store_wide_kernel(
     const __nv_bfloat16 *__restrict__ src, int lds, __nv_bfloat16 *__restrict__ q_out, int ldq, const int *__restrict__ positions, const int *__restrict__ cells,
     const int *__restrict__ seq_of_token, const int *__restrict__ block_table, int n_seqs, int max_blocks, const float *__restrict__ inv_freq,
     const float *__restrict__ inv_freq_lo, void *__restrict__ k_pages, void *__restrict__ v_pages, uint8_t *__restrict__ k_exps, uint8_t *__restrict__ v_exps,

@@ -46,8 +46,8 @@ def test_store_and_read_refuse_before_a_launch():
 @pytest.mark.parametrize("library,symbol", [("attention_tree", "lgml_tree_attention"), ("attention_tree_tall", "lgml_tree_attention_tall")])
 def test_attention_refuses_before_a_launch(library, symbol):
     p = P(0x1000)
-    good = [p, 512, p, p, p, None, p, 2, 4, p, p, p, p, 9, 64, p, 512, p, 1, 5, 4, 8, 2, 64, F(0.1), 0, p, None]
-    for change, what in (((14, 128), "pages of 128"), ((21, 7), "no multiple"), ((23, 40), "head_dim 40"), ((20, 0), "new tokens"), ((20, 65), "new tokens"), ((18, 0), "ranges"),
+    good = [p, 512, p, p, p, None, p, 2, 4, p, p, p, p, 9, 64, p, 512, p, 1, 5, 1, 4, 8, 2, 64, F(0.1), 0, p, None]
+    for change, what in (((14, 128), "pages of 128"), ((22, 7), "no multiple"), ((24, 40), "head_dim 40"), ((21, 0), "new tokens"), ((21, 65), "new tokens"), ((20, 0), "new tokens"), ((20, 5), "new tokens"), ((18, 0), "ranges"),
                          ((18, 257), "ranges"), ((11, None), "exponents"), ((9, P(0x1008)), "aligned"), ((1, 511), "aligned"), ((7, 1 << 30), "too many requests")):
         refused(library, symbol, at(change, size=good), what)
     refused(library, symbol, at((18, 9), (17, None), size=good), "scratch")
