@@ -3035,8 +3035,10 @@ def rope_kv_store(qkv, positions: torch.Tensor, seq_of_token: torch.Tensor, bloc
         lds = _rows_on(who, dev, src, "qkv", torch.bfloat16, width)
         n = src.shape[0]
     if q_out is None:
-        q_out = torch.empty((n, n_heads * head_dim), dtype=torch.bfloat16, device=src.device)
-    ldq = _rows_on(who, dev, q_out, "rotated q", torch.bfloat16, n_heads * head_dim, n)
+        ldq = n_heads * head_dim
+        q_out = src.new_empty((n, ldq), dtype=torch.bfloat16)
+    else:
+        ldq = _rows_on(who, dev, q_out, "rotated q", torch.bfloat16, n_heads * head_dim, n)
     _are(who, dev, torch.int32, 1, "positions, request index of tokens, cells, status", positions, seq_of_token, cells, status)
     _are(who, dev, torch.int32, 2, "block table", block_table)
     if positions.numel() != n or seq_of_token.numel() != n or (cells is not None and cells.numel() != n) or status.numel() != 1:
@@ -3077,13 +3079,16 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
     _are(who, dev, torch.int32, 1, "page list, status", pages, status)
     n = pages.numel()
     shape = (n, hkv, page, d)
+    if status.numel() != 1:
+        raise KernelError(f"{who}: the status is one int32")
     if k_out is None and v_out is None:
-        k_out, v_out = torch.empty((2,) + shape, dtype=torch.bfloat16, device=k_pages.device).unbind()
+        k_out, v_out = k_pages.new_empty((2,) + shape, dtype=torch.bfloat16).unbind()
     elif k_out is None or v_out is None:
         raise KernelError(f"{who}: results for the keys and the values, or for neither")
-    _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
-    if k_out.shape != shape or v_out.shape != shape or status.numel() != 1:
-        raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}, and the status is one int32")
+    else:
+        _are(who, dev, torch.bfloat16, 4, "keys read back, values read back", k_out, v_out)
+        if k_out.shape != shape or v_out.shape != shape:
+            raise KernelError(f"{who}: results are {shape}, not {tuple(k_out.shape)} and {tuple(v_out.shape)}")
     fn = _fn("kv_store", "lgml_kv_read", _READ_ARGS)
     _check("kv_store", fn(k_pages.data_ptr(), v_pages.data_ptr(), k_exps.data_ptr(), v_exps.data_ptr(), n_pages, page, pages.data_ptr(), n, k_out.data_ptr(),
                           v_out.data_ptr(), hkv, d, status.data_ptr(), _stream()), who)
@@ -3213,7 +3218,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int, status: to
     if not 0 <= top <= min(v, LOGPROBS_TOP) or v < 1:
         raise KernelError(f"{who}: {top} alternatives (0 to min(vocabulary {v}, {LOGPROBS_TOP}))")
     # all results in one allocation, each kind in one run: log p, rank, entropy, then ids and log p of the best
-    flat = torch.empty(n * (3 + 2 * top), dtype=torch.float32, device=logits.device)
+    flat = logits.new_empty(n * (3 + 2 * top))
     at = flat.data_ptr()
     fn = _fn("logprobs", "lgml_token_logprobs", _LOGPROBS_ARGS)
     _check("logprobs", fn(logits.data_ptr(), max(ld, v), n, v, ids.data_ptr(), int(top), _logprob_slices(n, v), at, at + 4 * n, at + 8 * n, at + 12 * n,
