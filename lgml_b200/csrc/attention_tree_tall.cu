@@ -27,6 +27,8 @@
 // Two tiles a block from 129 rows on, and a block an SM, against one tile and two blocks (us, each at its best cut; 2,064 cells, eight requests): 256 rows e4m3 38 / 58,
 // bfloat16 36 / 44, heads of 64 27 / 29; 132 rows e4m3 35 / 53, bfloat16 31 / 40; one request of 256 rows bfloat16 20 / 18; 512 rows, two of 8,256 cells: e4m3 61 / 89,
 // bfloat16 51 / 67.
+// That form is also the better one for a single tile where blocks have SMs to themselves (its second tile stays empty): 20 rows of one request e4m3 14.4 / 13.6 us, 108 of
+// one of 32,027 cells 82 / 61, bfloat16 46 / 43; not where two would share an SM: 36 rows of 64 requests of 1,009 cells 98 / 118.
 // Waits on mbarriers are bounded (status 14).
 #include "tree_common.cuh"
 
@@ -842,7 +844,14 @@ LGML_API int lgml_tree_attention_tall(const void *q, int ldq, const int *positio
     LGML_REQUIRE(ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0, "tree_attention: q and out must be 16-byte aligned here");
     LGML_REQUIRE((long long)n_seqs * (limit > n_splits ? limit : n_splits) <= 0x7fffffffLL, "tree_attention: too many requests");
     if (n_tokens == 0 || n_seqs == 0) return 0;
-    const int rows = limit * (H / Hkv), tiles = rows > ROWS ? 2 : 1;
+    static const int n_sms = [] {
+        int dev = 0, n = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        return n;
+    }();
+    // one block an SM, two tiles, deeper rings and more loaders: for more rows than a tile has, and where a block has an SM to itself anyway
+    const int rows = limit * (H / Hkv), tiles = rows > ROWS || (long long)n_seqs * n_splits * Hkv <= n_sms ? 2 : 1;
     const int n_chunks = (rows + tiles * ROWS - 1) / (tiles * ROWS);
     LGML_REQUIRE((long long)Hkv * n_chunks <= 65535, "tree_attention: too many heads");
     const int clustered = n_splits > 1 && n_splits <= MAX_CLUSTER;

@@ -3100,12 +3100,19 @@ def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int
     one kernel, more cost a second one (4 us) and are taken for 128 pages and more, of eight pages each.  (32 heads on 8 of 128, e4m3, us: one request of 1,001
     cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 52 in 8, 29 in 62; eight of 2,176 29, 17 in 6 to 8, 21 in
     16; 16 of 4,001 60, 30 in 4, 37 in 8; 64 of up to 4,097 85, 84 in 2, 120 in 8; 128 of 2,001 97, 107 in 2.  With 64 drafted tokens, four requests of up to 8,256
-    155, 84 in 2, 50 in 4, 88 in 8; 36 rows of eight requests of 2,009 73, 42 in 2, 31 in 4, 43 in 8.)"""
-    height, per_sm = (256, 1) if tall and rows > 128 else (128, 2) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
+    155, 84 in 2, 50 in 4, 88 in 8; 36 rows of eight requests of 2,009 50, 32 in 2, 31 in 4, 44 in 8; 108 rows of 16, bfloat16, 37, 50 in 2.)"""
+    height, per_sm = (256 if rows > 128 else 128, 1) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
     n = max(1, min(-(-pages // 2), (per_sm * sm_count()) // blocks, 64))
-    return n if n <= TREE_CLUSTER else TREE_CLUSTER if pages < 128 else max(TREE_CLUSTER, min(n, pages // 8))
+    if n > TREE_CLUSTER and pages >= 128:
+        return max(TREE_CLUSTER, min(n, pages // 8))
+    n = min(n, TREE_CLUSTER)
+    # A block an SM: clusters of 3 to 6 blocks find room on seven eighths of the SMs, of 7 and 8 on seven tenths (of 148: 135, 132, 130, 132, 105 and 120), and
+    # one cluster too many is a second wave (16 clusters of 8: 63 us, of 6: 41).
+    while tall and n > 2 and blocks * n > sm_count() * (7 if n <= 6 else 5.6) / 8:
+        n -= 1
+    return n
 
 
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
