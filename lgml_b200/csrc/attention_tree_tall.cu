@@ -7,6 +7,8 @@
 // tile's only chain is softmax after softmax.  (Products of one thread complete in the order of issue.)  Operands lie in shared memory in rows of 128 bytes,
 // swizzled; V is the N-major operand.  The running output stays in tensor memory; the softmax corrects it only when a row's maximum has grown by more than
 // 2^8 since its sums'.  The maximum is of the products as they are, so a score is one multiply-and-add; the scale has to be above zero.
+// P is rounded for the product, to float16 beside codes (half a step: 2^-12) and to bfloat16 beside bfloat16 (2^-9), as the types of a product must be; sums are float32, of
+// the probabilities before that (of the rounded bfloat16 ones, which attention_tree.cu takes: 3 to 10 % more time here).
 // Every mbarrier is of one stage, or one parity of pages, and what its next phase needs comes after its waiters have seen this one, so none is missed.
 // Tensor memory is taken behind the wait for the kernels ahead, so it is never held against one of them, and the kernels behind start when this one is done.
 //
