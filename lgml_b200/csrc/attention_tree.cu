@@ -19,7 +19,7 @@
 // e4m3: codes are exact in float16, so the products are of float16 (q is scaled per row by a power of two so that its largest
 // entry is in [2^14, 2^15): rounding it to float16 loses nothing above 2^-39 of that).  A key's power of two multiplies its score, exactly.  A value's joins
 // the probability's exponent: with w = log2 of the value's power, p'_c = exp2(score + w_c - m'), m' the maximum of score + w; p' is at most 1 and is
-// rounded to float16 (half a step: 2^-12), and the sum takes the rounded p' times 2^-w.  bfloat16: p is rounded to bfloat16 (2^-9), and the sum takes the rounded
+// rounded to float16 (half a step: 2^-11 of it), and the sum takes the rounded p' times 2^-w.  bfloat16: p is rounded to bfloat16 (2^-8), and the sum takes the rounded
 // ones.  Maxima, sums and outputs are float32.
 //
 // A value that is not finite must not reach a row that does not see it (0 x NaN): in blocks of 16 cells that not every row sees whole,

@@ -7,7 +7,7 @@
 // tile's only chain is softmax after softmax.  (Products of one thread complete in the order of issue.)  Operands lie in shared memory in rows of 128 bytes,
 // swizzled; V is the N-major operand.  The running output stays in tensor memory; the softmax corrects it only when a row's maximum has grown by more than
 // 2^8 since its sums'.  The maximum is of the products as they are, so a score is one multiply-and-add; the scale has to be above zero.
-// P is rounded for the product, to float16 beside codes (half a step: 2^-12) and to bfloat16 beside bfloat16 (2^-9), as the types of a product must be; sums are float32, of
+// P is rounded for the product, to float16 beside codes (half a step: 2^-11 of it) and to bfloat16 beside bfloat16 (2^-8), as the types of a product must be; sums are float32, of
 // the probabilities before that (of the rounded bfloat16 ones, which attention_tree.cu takes: 3 to 10 % more time here).
 // Every mbarrier is of one stage, or one parity of pages, and what its next phase needs comes after its waiters have seen this one, so none is missed.
 // Tensor memory is taken behind the wait for the kernels ahead, so it is never held against one of them, and the kernels behind start when this one is done.
@@ -24,7 +24,7 @@
 // rows of a page, and a page of two tiles takes 2,200 (the tensor cores are at work for 512 of them).  Two tiles a block convert a page once for 256 rows.
 // Three groups bring pages to two tiles, since sixteen warps are as many as leave a thread 128 registers.  Measured, four requests of up to 8,256 cells, 64
 // drafted tokens, 32 heads on 8 of 128, e4m3: 50 us (one tile a block, two threads a row, columns scaled one by one: 75; conversions by integer
-// arithmetic instead of the conversion instruction: 50; four groups at 96 registers: 59); 27 drafted tokens of one request over 2,203 cells, bfloat16: 15.6.
+// arithmetic instead of the conversion instruction: 50; four groups at 96 registers: 59); 27 drafted tokens of one request over 2,203 cells, bfloat16: 15.3.
 // Of those 50: 2 until the queries are in, 36 for 25 pages, 4 to join the ranges; the rest is blocks that start after others.
 // Two tiles a block from 129 rows on, and a block an SM, against one tile and two blocks (us, each at its best cut; 2,064 cells, eight requests): 256 rows e4m3 38 / 58,
 // bfloat16 36 / 44, heads of 64 27 / 29; 132 rows e4m3 35 / 53, bfloat16 31 / 40; one request of 256 rows bfloat16 20 / 18; 512 rows, two of 8,256 cells: e4m3 61 / 89,
