@@ -18,9 +18,11 @@
 //
 // e4m3: codes are exact in float16, so the products are of float16 (q is scaled per row by a power of two so that its largest
 // entry is in [2^14, 2^15): rounding it to float16 loses nothing above 2^-39 of that).  A key's power of two multiplies its score, exactly.  A value's joins
-// the probability's exponent: with w = log2 of the value's power, p'_c = exp2(score + w_c - m'), m' the maximum of score + w; p' is at most 1 and is
-// rounded to float16 (half a step: 2^-11 of it), and the sum takes the rounded p' times 2^-w.  bfloat16: p is rounded to bfloat16 (2^-8), and the sum takes the rounded
-// ones.  Maxima, sums and outputs are float32.
+// the exponent of its weight in the numerator: with w = log2 of the value's power, p'_c = 2^15 exp2(score + w_c - m'), m' the maximum of score + w, is
+// at most 2^15 and is rounded to float16: half a step, 2^-11 of it, down to 2^-29 of the largest, and 2^-40 of the largest under that.  The sum of the weights is another matter: a
+// value of zeros, or a small one, may have most of the weight, and beside it p' says nothing of that.  So it is of exp2(score - m) in float32, about a maximum of
+// the scores alone (every thread has one of its own, which needs no exchange), and the two meet at the end: o = exp2(m' - m) sum p' code / sum p.
+// bfloat16: p is rounded to bfloat16 (2^-8), and the sum takes the rounded ones.  Maxima, sums and outputs are float32.
 //
 // A value that is not finite must not reach a row that does not see it (0 x NaN): in blocks of 16 cells that not every row sees whole,
 // values are looked at, and where one is not finite the block's products are formed one by one.
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     float scale, int window, int *__restrict__ status) {
     pdl_trigger();
     constexpr int D = KS * 16, ROWS = 8 * NT;
+    constexpr float P_UP = Q8 ? 15.f : 0.f;               // the numerator's weights are times 2^this
     using C = Cut<KS, NT, Q8>;
     extern __shared__ __align__(16) uint8_t smem[];                // the warps' stages; at the end [WARPS][ROWS][D + 2] floats
     __shared__ int row_pos[ROWS];
@@ -214,9 +217,10 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 
     const float scale_log2 = scale * 1.4426950408889634f;
     float m_run[NT][2], l_run[NT][2], oacc[NT][KS][4];
+    float m_sum[NT][2];              // (e4m3) the maximum that l_run is about: of this thread's scores
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        m_run[nt][0] = m_run[nt][1] = -INFINITY, l_run[nt][0] = l_run[nt][1] = 0.f;
+        m_run[nt][0] = m_run[nt][1] = m_sum[nt][0] = m_sum[nt][1] = -INFINITY, l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; ++i) oacc[nt][i][0] = oacc[nt][i][1] = oacc[nt][i][2] = oacc[nt][i][3] = 0.f;
     }
@@ -282,7 +286,6 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
         }
         // ---- probabilities ----
         const float kf[2] = {Q8 ? scale_log2 * power_of_two(ke[0]) : scale_log2, Q8 ? scale_log2 * power_of_two(ke[1]) : scale_log2};
-        const float vf[2] = {Q8 ? power_of_two(-ve[0]) : 1.f, Q8 ? power_of_two(-ve[1]) : 1.f};
         unsigned pb0[NT], pb1[NT];
         bool grown = false;
         float corr[NT][2], pr[NT][4];
@@ -292,10 +295,22 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x = (SUMS == 2 ? sums[0][nt][i] + sums[SUMS - 1][nt][i] : sums[0][nt][i]) * kf[i >> 1];
-                if (Q8) x = x * q_unscale[nt][i & 1] + (float)ve[i >> 1];
+                if (Q8) x *= q_unscale[nt][i & 1];
                 sc[nt][i] = (seen[nt] >> i) & 1 ? x : -INFINITY;
-                mx[i & 1] = fmaxf(mx[i & 1], sc[nt][i]);
             }
+            if (Q8) {
+                // the weights, and then the scores with the values' powers
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float m_new = fmaxf(m_sum[nt][e], fmaxf(sc[nt][e], sc[nt][2 + e])), ref = m_new == -INFINITY ? 0.f : m_new;
+                    l_run[nt][e] = l_run[nt][e] * ex2(m_sum[nt][e] - ref) + (ex2(sc[nt][e] - ref) + ex2(sc[nt][2 + e] - ref));
+                    m_sum[nt][e] = m_new;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[nt][i] += (float)ve[i >> 1];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i & 1] = fmaxf(mx[i & 1], sc[nt][i]);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
@@ -305,12 +320,12 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
                 corr[nt][e] = m_new == m_run[nt][e] ? 1.f : ex2(m_run[nt][e] - m_new);
                 grown |= m_new != m_run[nt][e];
                 m_run[nt][e] = m_new;
-                l_run[nt][e] *= corr[nt][e];
+                if (!Q8) l_run[nt][e] *= corr[nt][e];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float m = m_run[nt][i & 1];
-                pr[nt][i] = ex2(sc[nt][i] - (m == -INFINITY ? 0.f : m));          // (unseen: exp2(-inf) = 0)
+                pr[nt][i] = ex2(sc[nt][i] - (m == -INFINITY ? 0.f : m - P_UP));          // (unseen: exp2(-inf) = 0)
             }
             unsigned lo, hi;
             if (Q8) {
@@ -324,8 +339,9 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
                 const float2 fa = __bfloat1622float2(a), fb = __bfloat1622float2(b);
                 pr[nt][0] = fa.x, pr[nt][1] = fa.y, pr[nt][2] = fb.x, pr[nt][3] = fb.y;
             }
+            if (!Q8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l_run[nt][i & 1] += pr[nt][i] * vf[i >> 1];
+                for (int i = 0; i < 4; ++i) l_run[nt][i & 1] += pr[nt][i];
             pb0[nt] = transpose8(lo);
             pb1[nt] = transpose8(hi);
         }
@@ -412,7 +428,16 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float l = l_run[nt][e];
+            float l = l_run[nt][e], m = m_run[nt][e], up = 1.f;
+            if (Q8) {
+                // the eight threads' sums about one maximum m, and the outputs about the same; both times 2^-24, so that sums of the largest values stay finite
+                m = fmaxf(m_sum[nt][e], __shfl_xor_sync(0xffffffffu, m_sum[nt][e], 4));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                const bool none = m == -INFINITY;
+                l *= ex2((none ? 0.f : m_sum[nt][e] - m) - 24.f);
+                up = none ? 1.f : ex2(m_run[nt][e] - m - P_UP - 24.f);
+            }
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
@@ -420,9 +445,9 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
 #pragma unroll
             for (int mt = 0; mt < KS; ++mt) {
                 const int d = C::value_entry(mt, g);
-                *reinterpret_cast<float2 *>(row + d) = make_float2(oacc[nt][mt][e], oacc[nt][mt][2 + e]);
+                *reinterpret_cast<float2 *>(row + d) = Q8 ? make_float2(oacc[nt][mt][e] * up, oacc[nt][mt][2 + e] * up) : make_float2(oacc[nt][mt][e], oacc[nt][mt][2 + e]);
             }
-            if (g == 0) *reinterpret_cast<float2 *>(row + D) = make_float2(m_run[nt][e], l);
+            if (g == 0) *reinterpret_cast<float2 *>(row + D) = make_float2(m, l);
         }
     __syncthreads();
     for (int i = tid; i < ROWS * (D / 2); i += THREADS) {
