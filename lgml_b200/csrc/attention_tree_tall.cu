@@ -8,7 +8,8 @@
 // swizzled; V is the N-major operand.  The running output stays in tensor memory; the softmax corrects it only when a row's maximum has grown by more than
 // 2^8 since its sums'.  The maximum is of the products as they are, so a score is one multiply-and-add; the scale has to be above zero.
 // P is rounded for the product, to float16 beside codes (half a step: 2^-11 of it) and to bfloat16 beside bfloat16 (2^-8), as the types of a product must be; sums are float32, of
-// the probabilities before that (of the rounded bfloat16 ones, which attention_tree.cu takes: 3 to 10 % more time here).
+// the probabilities before that (of the rounded bfloat16 ones, which attention_tree.cu takes: 3 to 10 % more time here).  Beside codes a probability is times its value's
+// power of two, so the sum is about a maximum of its own, of the scores alone: powers that are 2^100 apart, or values of zeros, take nothing from it.
 // Every mbarrier is of one stage, or one parity of pages, and what its next phase needs comes after its waiters have seen this one, so none is missed.
 // Tensor memory is taken behind the wait for the kernels ahead, so it is never held against one of them, and the kernels behind start when this one is done.
 //
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
     int ldo, float *__restrict__ part_o, float2 *__restrict__ part_ml, int n_splits, int clustered, int n_tokens, int H, int Hkv, int n_chunks, int least, int limit,
     float scale, int window, int *__restrict__ status) {
     constexpr int KB = D / 64;                        // 64-element blocks along the head
-    constexpr float P_UP = Q8 ? 7.f : 0.f;            // probabilities times 2^this, in the products and the sums: at most 2^15, float16 has numbers down to 2^-24
+    constexpr float P_UP = Q8 ? 7.f : 0.f;            // probabilities times 2^this in the products: at most 2^15, float16 has numbers down to 2^-24
     using R = Roles<TILES, Q8>;
     constexpr int THREADS = R::THREADS, LOADERS = R::LOADERS, GROUPS = R::GROUPS, STAGES = R::STAGES, ALL_ROWS = TILES * ROWS;
     constexpr uint32_t Q_BYTES = KB * ROWS * 128, K_BYTES = KB * PAGE * 128;          // of a tile's queries, of a page's keys
@@ -237,8 +238,7 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *Qs = base, *Ks = Qs + TILES * Q_BYTES, *Vs = Ks + STAGES * K_BYTES;
     constexpr int RING = 2 * STAGES;                      // pages whose columns are described (a page is described again when the softmax of RING pages before is done)
-    __shared__ __align__(16) float kf_s[RING][PAGE], add_s[RING][PAGE], vf_s[RING][PAGE];      // per column of page it (it % RING): its scores' factor, what is
-                                                                                               // added to them, and what its probability counts for in the sum
+    __shared__ __align__(16) float kf_s[RING][PAGE], add_s[RING][PAGE];      // per column of page it (it % RING): its scores' factor, its value's power of two
     __shared__ __align__(8) float fin[ALL_ROWS][2];
     __shared__ int unscale_s[ALL_ROWS];                   // q was multiplied by 2 to the minus this
     __shared__ __align__(16) int4 page_s[RING];           // of page it: the powers of two its keys and its values were divided by, whether they are in column by
@@ -435,7 +435,6 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
                 const int ke = (l < 32 ? k0 : k1) - 127, ve = (l < 32 ? v0 : v1) - 127;
                 kf_s[it % RING][l] = scale_log2 * power_of_two(max(ke, -126));
                 add_s[it % RING][l] = (float)ve;
-                vf_s[it % RING][l] = power_of_two(-ve);
             }
         }
         return keys ? Powers{k_largest, {k0, k1}, apart} : Powers{v_largest, {v0, v1}, apart};
@@ -456,7 +455,8 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
             if (l + LOADERS * u < PAGE * D * SIZE / 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (size_t)(l + LOADERS * u) * 128));
     };
     const uint32_t ks0 = smem_u32(Ks), vs0 = smem_u32(Vs);
-    float m_ref = -INFINITY, l_run = 0.f;
+    // Output and sum are about maxima of their own where pages hold codes: m_ref is of scores and their values' powers together, m_sum of the scores alone.
+    float m_ref = -INFINITY, m_sum = -INFINITY, l_run = 0.f, up = 1.f;
     if (tid >= R::BRING && tid < R::ISSUERS) {
         // ---- the keys and the values: a stage is free when the products of the page that was in it have read it ----
         // (page numbers come ahead and ask L2 for their pages, codes and exponents set out as what is before them goes in: each is a trip to L2 or beyond)
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
             tcgen05_ld_32(s_addr + 32u, *reinterpret_cast<uint32_t(*)[32]>(&r.u[32]));
             tcgen05_wait_ld();
             // a score (in powers of two, of what the values are multiplied by too) is r times + plus
-            float times = scale_log2, plus = 0.f, back = 1.f;
+            float times = scale_log2, plus = 0.f;
             if (Q8) {
                 if (page.z) {
                     // (rare) column by column
@@ -619,7 +619,6 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
                 } else {
                     times = scale_log2 * power_of_two(min(max(page.x + unscale, -120), 120));
                     plus = (float)page.y;
-                    back = power_of_two(-page.y);
                 }
             }
             if (edge) {
@@ -632,14 +631,28 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < PAGE; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(r.u[c]), __uint_as_float(r.u[c + 1]));
-            const float m_new = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), times, plus);
+            const float largest = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_new = fmaf(largest, times, plus);
+            if (Q8) {
+                float s_new = largest * times;
+                if (page.z) {
+                    s_new = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < PAGE; ++c) s_new = fmaxf(s_new, __uint_as_float(r.u[c]) - add_s[it % RING][c]);
+                }
+                if (m_sum == -INFINITY) {
+                    m_sum = s_new;
+                } else if (s_new > m_sum + RESCALE_STEP) {
+                    l_run *= ex2(m_sum - s_new);
+                    m_sum = s_new;
+                }
+            }
             float corr = 1.f;
             if (m_ref == -INFINITY) {
                 m_ref = m_new;                       // nothing summed yet: nothing to correct
             } else if (m_new > m_ref + RESCALE_STEP) {
                 corr = ex2(m_ref - m_new);
                 m_ref = m_new;
-                l_run *= corr;
+                if (!Q8) l_run *= corr;
             }
             if (__any_sync(0xffffffffu, corr != 1.f)) {
                 // ---- correct the running output (rare): the product of the page before must be done, this page's has to wait for P ----
@@ -677,18 +690,31 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
                 tcgen05_st_16(s_addr + (uint32_t)c0, packed);
             }
             float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-            if (Q8 && page.z) {
-                sum = 0.f;
+            if (Q8) {
+                // The probabilities come with their values' powers: one factor takes those out again, unless they differ by column, or leave too little of them.
+                const float ref = m_sum == -INFINITY ? 0.f : m_sum;
+                const bool little = m_new < m_ref - 60.f;
+                if (page.z || (little && m_new > -INFINITY)) {
+                    sum = 0.f;
 #pragma unroll
-                for (int c = 0; c < PAGE; ++c) sum = fmaf(ex2(__uint_as_float(r.u[c]) + less), vf_s[it % RING][c], sum);
+                    for (int c = 0; c < PAGE; ++c) sum += ex2(fmaf(__uint_as_float(r.u[c]), times, -ref) - (page.z ? add_s[it % RING][c] : 0.f));
+                } else if (!little) {             // (little of nothing seen: 0, whatever the factor)
+                    sum *= ex2((m_ref == -INFINITY ? 0.f : m_ref) - plus - P_UP - ref);
+                }
             }
-            l_run = fmaf(sum, back, l_run);
+            l_run += sum;
             tcgen05_wait_st();
             tcgen05_fence_before();
             warp_arrive(&p_full[tile][it & 1]);
         }
         // (the last scores were seen, and were issued behind the product two pages before: the barrier is at most a phase away)
         if (n_it > 0 && alive && !mbar_wait(&o_done[tile][(n_it - 1) & 1], ((n_it - 1) >> 1) & 1, abort_flag, status)) alive = false;
+        if (Q8) {
+            // (both times 2^-24, so that sums of the largest values stay finite)
+            if (m_sum != -INFINITY) up = ex2(m_ref - m_sum - P_UP - 24.f);
+            m_ref = m_sum;
+            l_run *= 5.9604644775390625e-8f;
+        }
         fin[row][0] = m_ref;
         fin[row][1] = l_run;
     }
@@ -711,6 +737,9 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
             if (n_it > 0) {
                 tcgen05_ld_16(lane_addr + O_COL + (uint32_t)c0, r);
                 tcgen05_wait_ld();
+                if (Q8)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * up);
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) r[j] = 0u;

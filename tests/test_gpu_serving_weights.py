@@ -54,3 +54,23 @@ def test_a_cell_of_zeros_that_has_most_of_the_weight(shape):
         p.ke[row[0], :, 0] = 127
     for n_splits in (None, 1, 5, 12):
         p.check(p.run(n_splits=n_splits))
+
+
+@pytest.mark.parametrize("whole_pages", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_weights_beside_values_near_the_end_of_the_range(shape, whole_pages):
+    """Values of about 2^100, beside zeros and beside values 2^60 and 2^140 smaller: in the same page, and in pages of their own."""
+    for by in (None, 60, 140):
+        p = problem(shape, 0.3, seed=2)
+        p.ve.copy_((p.ve.int() + 100).clamp(67, 246).to(torch.uint8))
+        if whole_pages:
+            for row in p.table:
+                for page in row[1::2] if len(row) > 3 else row[:1]:
+                    if page >= 0:
+                        if by is None:
+                            p.v.view(torch.uint8)[page] = 0
+                        p.ve[page] = 67 if by is None else (p.ve[page].int() - by).clamp(67, 246).to(torch.uint8)
+        else:
+            shrink(p, slice(1, None, 2), by)
+        for n_splits in (1, 3, 12):
+            p.check(p.run(n_splits=n_splits))
