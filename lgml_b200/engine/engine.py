@@ -168,6 +168,8 @@ class Engine:
             rec["toks"] = [int(e.request.sampler.sample_candidates(ids[i], vals[i])) for i, e in enumerate(rows)]
         else:
             host_logits = logits.cpu().numpy()
+            if self._logprobs is not None and any(e.request.params.edits_logits for e in rows):
+                logits = self._apply_edits(logits, rows)        # (the scores are of these; the host's chain edits the rows it was given)
             rec["toks"] = [int(e.request.sampler.sample(host_logits[i])) for i, e in enumerate(rows)]
         if self._logprobs is not None:
             ids = rec["out"] if rec["toks"] is None else torch.tensor(rec["toks"], dtype=torch.int32).to(logits.device)

@@ -1,0 +1,47 @@
+"""What the engine gives with log probabilities and with drafted tokens, where the plain calls of ``test_gpu_eight_bit_cache.py`` do not look."""
+import math
+
+import pytest
+import torch
+
+from tests import helpers as H
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def folder(tmp_path_factory):
+    return H.make_folder(tmp_path_factory.mktemp("serving"), H.TINY_B, 1, dtype="float32")
+
+
+EDITS = dict(repeat_penalty=1.4, frequency_penalty=0.3, presence_penalty=0.2, logit_bias={5: 6.0, 9: -4.0, 11: -math.inf, 17: 5.5})
+
+
+@pytest.mark.parametrize("common,per_prompt", [
+    (dict(temperature=0.0), None), (dict(temperature=0.8, seed=3, top_k=0, top_p=0.9), None), (dict(temperature=0.8, seed=4, top_k=200), None), (dict(temperature=0.8, seed=5, top_k=20), None),
+    (dict(temperature=0.8, seed=6, **EDITS), [dict(top_k=20), dict(top_k=7), dict(temperature=0.0)])])
+def test_scores_are_of_the_distribution_behind_bias_and_penalties(folder, common, per_prompt):
+    """Logits of this engine in float32 are within 2e-4 of the plain implementation's; a penalty makes that 1.4 times as much, a difference of two of
+    them twice that: 6e-4, and the entropy's weighted mean of log probabilities is as far off."""
+    import lgml_b200
+
+    eng = lgml_b200.Engine(str(folder), dtype="float32", slots=3)
+    prompts = [H.random_ids(n, 320, n) for n in (3, 20, 9)]
+    got = eng.generate(prompts, max_tokens=8, logprobs=4, per_prompt=per_prompt, **{**EDITS, **common})
+    for p, (ids, scores) in zip(prompts, got):
+        assert len(ids) == len(scores) == 8
+        logits = H.oracle_logits(folder, p + ids).double()
+        for i, sc in enumerate(scores):
+            row = logits[len(p) + i - 1].clone()
+            for t, b in EDITS["logit_bias"].items():
+                row[t] += b
+            for t in set(ids[:i]):
+                row[t] = row[t] * 1.4 if row[t] <= 0 else row[t] / 1.4
+                row[t] -= ids[:i].count(t) * 0.3 + 0.2
+            logs = torch.log_softmax(row, -1)
+            assert sc.id == ids[i] and abs(sc.logprob - logs[ids[i]]) <= 1e-3, (i, sc, float(logs[ids[i]]))
+            weighted = torch.where(logs == -math.inf, torch.zeros_like(logs), logs.exp() * logs)
+            assert abs(sc.entropy + weighted.sum()) <= 3e-3
+            order = torch.argsort(row, descending=True)
+            assert len(sc.top) == 4 and all(abs(lp - logs[t]) <= 1e-3 and lp >= float(logs[order[j]]) - 2e-3 for j, (t, lp) in enumerate(sc.top))
+            assert abs(float(logs[order[sc.rank]] - logs[ids[i]])) <= 2e-3
