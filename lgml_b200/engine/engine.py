@@ -144,7 +144,7 @@ class Engine:
                 us = torch.tensor([0.0 if e.request.params.greedy else e.request.sampler.uniform() for e in rows],
                                   dtype=torch.float64).pin_memory()
                 ops.sample_rows(logits, temps.to(logits.device, non_blocking=True), us.to(logits.device, non_blocking=True), out)
-            self._ids_to_host(rec, out)
+            rec["out"] = out
         elif n <= MAX_RESULT and self._candidates_on_device(rows, logits.shape[1]):
             # top_k, then the rest of the chain on its candidates, all on the device: the ids stay
             # there for the next step, as with the argmax
@@ -156,7 +156,7 @@ class Engine:
             res = self.rt.result
             out = res[MAX_RESULT - n:MAX_RESULT]
             ops.sample_candidates(vals, ids, params.to(logits.device, non_blocking=True), us.to(logits.device, non_blocking=True), out)
-            self._ids_to_host(rec, out)
+            rec["out"] = out
         elif all(e.request.params.top_k_on_device and e.request.params.top_k == rows[0].request.params.top_k for e in rows) \
                 and rows[0].request.params.top_k < logits.shape[1]:
             # bias, penalties and top_k on the device; the host runs the rest of the chain on k
@@ -174,6 +174,8 @@ class Engine:
         if self._logprobs is not None:
             ids = rec["out"] if rec["toks"] is None else torch.tensor(rec["toks"], dtype=torch.int32).to(logits.device)
             rec["scores"] = PendingScores(logits, ids, self._logprobs, self.rt.status)
+        if rec["toks"] is None:
+            self._ids_to_host(rec, rec["out"])          # (behind the scores: the status word travels with the ids)
         return rec
 
     def _ids_to_host(self, rec: dict, out: torch.Tensor) -> None:
@@ -184,7 +186,7 @@ class Engine:
         host[:n + 1].copy_(self.rt.result[MAX_RESULT - n:], non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
-        rec.update(out=out, host=host, event=ev)
+        rec.update(host=host, event=ev)
 
     @staticmethod
     def _candidates_on_device(rows, vocab: int) -> bool:

@@ -45,3 +45,23 @@ def test_scores_are_of_the_distribution_behind_bias_and_penalties(folder, common
             order = torch.argsort(row, descending=True)
             assert len(sc.top) == 4 and all(abs(lp - logs[t]) <= 1e-3 and lp >= float(logs[order[j]]) - 2e-3 for j, (t, lp) in enumerate(sc.top))
             assert abs(float(logs[order[sc.rank]] - logs[ids[i]])) <= 2e-3
+
+
+@pytest.mark.parametrize("options", [dict(temperature=0.0), dict(temperature=0.8, seed=1, top_k=20), dict(temperature=0.8, seed=1, top_k=0, top_p=0.9)])
+def test_a_status_that_the_scores_set_is_of_their_own_step(folder, options, monkeypatch):
+    """The status word as the kernel would leave it after its copies' time ran out."""
+    import lgml_b200
+    from lgml_b200 import ops
+
+    eng = lgml_b200.Engine(str(folder), dtype="float32", slots=1)
+    plain = ops.token_logprobs
+
+    def timed_out(logits, ids, top, status):
+        got = plain(logits, ids, top, status)
+        status.fill_(15)
+        return got
+
+    monkeypatch.setattr(ops, "token_logprobs", timed_out)
+    with pytest.raises(RuntimeError, match="log probabilities"):
+        eng.generate([[1, 2, 3]], max_tokens=1, logprobs=2, **options)
+    assert eng.rt.status.item() == 0
