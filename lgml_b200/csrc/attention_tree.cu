@@ -111,9 +111,11 @@ __global__ void __launch_bounds__(THREADS) tree_attention_kernel(
     // (the step's description, down to the first pages' numbers, is read while the kernels ahead may still run)
     const int row0 = early_int(seq_start + s), n = early_int(seq_start + s + 1) - row0, pos0 = early_int(seq_pos0 + s);
     const int group = H / Hkv, n_rows = n * group, r0 = chunk * ROWS;
-    if (n < least || n > limit || r0 >= n_rows) return;
-    if (row0 < 0 || row0 + n > n_tokens || pos0 < 0) {
-        if (tid == 0) atomicExch(status, 3);
+    // (A block that leaves waits first: a grid none of whose blocks waited could be over before the kernels ahead are, and the kernel behind waits for this grid alone.)
+    const bool misplaced = row0 < 0 || row0 + n > n_tokens || pos0 < 0;
+    if (n < least || n > limit || r0 >= n_rows || misplaced) {
+        pdl_wait();
+        if (misplaced && n >= least && n <= limit && tid == 0) atomicExch(status, 3);
         return;
     }
     if (tid < ROWS) {
