@@ -323,6 +323,10 @@ class CacheManager:
                 worst = max(worst, need - len(req.tables[gi]))
         return max(worst, 0)
 
+    def cells_left(self, req: Request) -> int:
+        """New tokens that ``reserve`` can give cells to now: the rest of the pages that the request holds, and the free ones."""
+        return min(((len(req.tables[gi]) + grp.pool.n_free) * self.page_size for gi, grp in enumerate(self.groups)), default=1 << 30) - req.n_tokens
+
     def reserve(self, req: Request, n_new: int) -> bool:
         """Take the pages that positions [n_tokens, n_tokens + n_new) need, in every group,
         or none at all.  False when a pool cannot give them."""

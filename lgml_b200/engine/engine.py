@@ -28,7 +28,7 @@ import torch
 from .. import ops
 from ..cache import PAGE_SIZE
 from ..sampling import Sampler, SamplingParams, log_min_p
-from .runner import ModelRunner
+from .runner import ModelRunner, StepError
 from .runtime import MAX_RESULT
 from .scores import PendingScores, TokenScore
 from .scheduler import REPEAT_STOP, UBATCH, GenRequest, Scheduler
@@ -378,6 +378,24 @@ class Engine:
             out.append(mine)
         return out
 
+    @staticmethod
+    def _drafts(draft, ids: List[int], wanted: int):
+        """What ``draft`` gives behind ``ids``, without the tokens that lie so deep that ``wanted`` new ones are there before them."""
+        tokens, parents = (list(x) for x in draft(ids))
+        if len(tokens) != len(parents):
+            raise StepError(f"greedy: {len(tokens)} drafted tokens and {len(parents)} parents")
+        kept, links, depth, place = [], [], [], {-1: -1}
+        for i, (t, p) in enumerate(zip(tokens, parents)):
+            p = max(int(p), -1)
+            if p >= i:
+                raise StepError(f"greedy: drafted token {i} follows token {p}, which is not before it")
+            depth.append(1 if p < 0 else depth[p] + 1)
+            if depth[i] < wanted:
+                place[i] = len(kept)
+                kept.append(int(t))
+                links.append(place[p])
+        return kept, links
+
     def greedy(self, prompt: Sequence[int], n_predict: int, stop: Optional[Sequence[int]] = None, draft=None):
         """Greedy decode of one prompt: (new ids, timings {prefill, decode, n_decode, steps}), as
         ``generate.greedy`` (``lua/lgml/generate.lua:19-34``).  With ``draft`` (a callable as in ``engine/drafts.py``: ids so far -> tokens, parents) every
@@ -415,9 +433,10 @@ class Engine:
                     cur = int(ops.argmax_rows(logits, tok).item())
                     out.append(cur)
                     continue
-                drafted, parents = draft(prompt + out)
-                room = min(ops.TREE_TOKENS, self.scheduler.max_position - req.n_tokens) - len(chain)
-                drafted, parents = [int(t) for t in drafted][:max(room, 0)], [int(p) for p in parents][:max(room, 0)]
+                drafted, parents = self._drafts(draft, prompt + out, n_predict - len(out))
+                # (drafts take cells that are there: a pool that the tokens alone fill gives them none)
+                room = min(ops.TREE_TOKENS, self.scheduler.max_position - req.n_tokens, runner.cache.cells_left(req)) - len(chain)
+                drafted, parents = drafted[:max(room, 0)], parents[:max(room, 0)]
                 m = len(chain)
                 tokens = chain + drafted
                 logits = runner.step_tree([(req, tokens, list(range(-1, m - 1)) + [m - 1 if p < 0 else m + p for p in parents])])

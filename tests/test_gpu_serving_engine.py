@@ -65,3 +65,29 @@ def test_a_status_that_the_scores_set_is_of_their_own_step(folder, options, monk
     with pytest.raises(RuntimeError, match="log probabilities"):
         eng.generate([[1, 2, 3]], max_tokens=1, logprobs=2, **options)
     assert eng.rt.status.item() == 0
+
+
+@pytest.mark.parametrize("name", ["B", "C"])
+@pytest.mark.parametrize("cache_dtype", [None, "float8_e4m3"])
+def test_drafts_need_no_more_room_than_the_tokens(tmp_path, name, cache_dtype):
+    """A pool of two pages that plain greedy decoding fills but for one cell, and drafters that would have more."""
+    import lgml_b200
+    from tests.test_gpu_eight_bit_cache import consistent
+
+    config, seed = H.TINY[name]
+    folder = H.make_folder(tmp_path, config, seed, dtype="bfloat16", sharpen=3.0)
+    vocab = config["vocab_size"]
+    eng = lgml_b200.Engine(str(folder), cache_dtype=cache_dtype, slots=1, kv_tokens=128)
+    prompt = H.random_ids(45, vocab, 8)
+    plain, _ = eng.greedy(prompt, 83)
+    assert len(plain) == 83
+
+    def right(ids):
+        more = plain[len(ids) - len(prompt):][:30]
+        return more + [1] * 20, [-1] + list(range(len(more) - 1)) + [-1] * 20 if more else [-1] * 20
+
+    for draft in (right, lambda ids: (H.random_ids(63, vocab, len(ids)), [-1] * 63), lambda ids: (H.random_ids(63, vocab, len(ids)), list(range(-1, 62)))):
+        got, t = eng.greedy(prompt, 83, draft=draft)
+        assert len(got) == 83 and t["steps"] <= 82
+        consistent(eng, prompt, got)
+        assert not eng.runner.cache.live and eng.runner.cache.n_free_pages == eng.runner.cache.n_pages
