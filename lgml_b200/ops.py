@@ -3115,6 +3115,11 @@ def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int
     return n
 
 
+def _tree_is_tall(rows: int, kv_heads: int, d: int, eight: bool, scale: float, q: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether ``rows`` rows of each of the requests' KV heads go to the tcgen05 kernel (which takes a row's maximum before it scales)."""
+    return rows >= TREE_TALL_ROWS[eight and kv_heads > sm_count()] and d in (64, 128) and scale > 1e-6 and prefill_tc_supports(q, out)
+
+
 def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
                    v_pages: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, window: int, status: torch.Tensor, max_new_tokens: int,
                    max_kv_len: int, k_exps: Optional[torch.Tensor] = None, v_exps: Optional[torch.Tensor] = None, visible: Optional[torch.Tensor] = None,
@@ -3149,8 +3154,7 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
         if visible.numel() != n:
             raise KernelError(f"{who}: one mask a token")
     rows = max_new_tokens * (n_heads // hkv)
-    # (the tcgen05 kernel takes a row's maximum before it scales)
-    tall = rows >= TREE_TALL_ROWS[k_exps is not None and seqs * hkv > sm_count()] and d in (64, 128) and scale > 1e-6 and ldq % 8 == 0 and ldo % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
+    tall = _tree_is_tall(rows, seqs * hkv, d, k_exps is not None, scale, q, out)
     if n_splits is None:
         n_splits = tree_splits(seqs, hkv, rows, max_kv_len if not window else min(max_kv_len, window + max_new_tokens + page), page, tall)
     if n_splits > TREE_CLUSTER:
@@ -3175,6 +3179,8 @@ def cached_attention(q, batch, cache, out, n_heads: int, scale: float, window: i
     visible = getattr(batch, "visible", None)
     table, k, v = cache.block_table, cache.k, cache.v
     short = [n for n in batch.seq_lens if n <= TREE_TOKENS]
+    if visible is not None and len(short) < len(batch.seq_lens):
+        raise KernelError(f"cached_attention: a tree has at most {TREE_TOKENS} tokens, a request brings {batch.max_q_len}")
     # Many requests of a token or a few beside one of many: each kind by the kernel that suits its rows (a block of 256 rows takes three times as long over a single
     # token's four as one of eight does: 64 requests of up to 4,096 cells beside one of 64 new tokens 331 us in one call, 136 in two; 20 of them 154 and 64).
     few = [n for n in short if n * (n_heads // k.shape[1]) < TREE_TALL_ROWS[0]]
@@ -3185,13 +3191,12 @@ def cached_attention(q, batch, cache, out, n_heads: int, scale: float, window: i
         splits = None
         if len(parts) > 1:      # (ranges for the requests of this part)
             rows, longest = max(lens) * (n_heads // k.shape[1]), batch.max_kv_len if not window else min(batch.max_kv_len, window + max(lens) + k.shape[2])
-            splits = tree_splits(len(lens), k.shape[1], rows, longest, k.shape[2], tall=rows >= TREE_TALL_ROWS[0] and k.shape[3] in (64, 128))
+            tall = _tree_is_tall(rows, len(batch.seq_lens) * k.shape[1], k.shape[3], cache.k_exps is not None, scale, q, out)
+            splits = tree_splits(len(lens), k.shape[1], rows, longest, k.shape[2], tall)
         tree_attention(q, batch.positions, batch.seq_start, batch.seq_pos0, table, k, v, out, n_heads, scale, window, status, max_new_tokens=max(lens),
                        max_kv_len=batch.max_kv_len, k_exps=cache.k_exps, v_exps=cache.v_exps, visible=visible, n_splits=splits, min_new_tokens=least)
     if len(short) == len(batch.seq_lens):
         return out
-    if visible is not None:
-        raise KernelError(f"cached_attention: a tree has at most {TREE_TOKENS} tokens, a request brings {batch.max_q_len}")
     d, hkv = k.shape[3], k.shape[1]
     pages, table = batch.read_back(cache.group, TREE_TOKENS)
     k, v = kv_read(k, v, cache.k_exps, cache.v_exps, pages, status)

@@ -39,3 +39,41 @@ def test_drafts_that_lie_too_deep_are_left_out():
     for bad in (([1, 2], [-1]), ([1, 2], [0, -1]), ([1, 2], [-1, 1])):
         with pytest.raises(StepError):
             Engine._drafts(lambda ids: bad, [1], 5)
+
+
+def cached(monkeypatch, lens, calls, visible=None, group=4, dim=64):
+    """The calls of ``tree_attention`` that ``cached_attention`` makes for requests that bring these numbers of tokens, over e4m3 pages of two KV heads."""
+    from types import SimpleNamespace
+
+    from lgml_b200 import ops
+
+    monkeypatch.setattr(ops, "sm_count", lambda: 148)
+    monkeypatch.setattr(ops, "tree_attention", lambda *a, **kw: calls.append(kw))
+    H, G, N = 2 * group, 2, sum(lens)
+    q = torch.zeros(N, H * dim, dtype=torch.bfloat16)
+    pages = torch.zeros(1, G, 64, dim, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    exps = torch.zeros(1, G, 64, dtype=torch.uint8)
+    batch = SimpleNamespace(positions=None, seq_start=None, seq_pos0=None, seq_lens=lens, max_kv_len=4000, max_q_len=max(lens), visible=visible)
+    cache = SimpleNamespace(block_table=None, k=pages, v=pages, k_exps=exps, v_exps=exps)
+    ops.cached_attention(q, batch, cache, torch.empty_like(q), H, 0.1, 0, None)
+    return calls
+
+
+@pytest.mark.parametrize("tokens,tall", [(5, False), (8, False), (9, True), (64, True)])
+def test_ranges_are_planned_for_the_kernel_that_runs(monkeypatch, tokens, tall):
+    """Many decoded tokens beside portions of 17 to 32 rows a KV head, which e4m3 pages of more KV heads than SMs leave to the few rows' kernel, and of more."""
+    from lgml_b200 import ops
+
+    first, second = cached(monkeypatch, [1] * 80 + [tokens] * 20, [])
+    assert (first["max_new_tokens"], first["min_new_tokens"], second["max_new_tokens"], second["min_new_tokens"]) == (1, 1, tokens, 2)
+    cuts = {t: ops.tree_splits(20, 2, 4 * tokens, 4000, 64, tall=t) for t in (False, True)}
+    assert second["n_splits"] == cuts[tall] and (tall or cuts[True] != cuts[False])
+
+
+def test_a_tree_of_too_many_tokens_is_refused_before_anything_is_launched(monkeypatch):
+    from lgml_b200 import ops
+
+    calls = []
+    with pytest.raises(ops.KernelError, match="64 tokens"):
+        cached(monkeypatch, [3, 65], calls, visible=object())
+    assert not calls and len(cached(monkeypatch, [3, 64], calls, visible=object())) == 1
