@@ -203,6 +203,7 @@ class ModelRunner:
         wanted).  Returns float32 [wanted, vocab] in the order of entries and places."""
         brought = self.validate(entries)
         self._reserve_all([(req, len(tokens)) for req, tokens, _ in entries])
+        self._forget_drafts([e[0] for e in entries])
         stage = self._pinned[self.steps % len(self._pinned)]
         if stage[1] is not None:
             stage[1].synchronize()
@@ -332,6 +333,7 @@ class ModelRunner:
         whole = [(req, tokens, range(len(tokens))) for req, tokens, _ in entries]
         brought = self.validate(whole)
         self._reserve_all([(req, len(tokens)) for req, tokens, _ in entries])
+        self._drafted = {}
         stage = self._pinned[self.steps % len(self._pinned)]
         if stage[1] is not None:
             stage[1].synchronize()
@@ -344,6 +346,12 @@ class ModelRunner:
         self.steps += 1
         self.tokens_run += sum(len(e[1]) for e in entries)
         return logits
+
+    def _forget_drafts(self, requests: Sequence[Request]) -> None:
+        """A step of these requests writes over the cells of their drafted tokens, also where it then fails."""
+        if self._drafted:
+            for req in requests:
+                self._drafted.pop(req, None)
 
     def keep(self, req: Request, n: int) -> None:
         """The first ``n`` tokens that the last ``step_tree`` ran for the request stay in its cache: each must follow the one before it."""
@@ -366,6 +374,7 @@ class ModelRunner:
         entries = [(r, [0], [0]) for r in requests]
         self.validate(entries)
         self._reserve_all([(r, 1) for r in requests])
+        self._forget_drafts(requests)
         stage = self._pinned[self.steps % len(self._pinned)]
         if stage[1] is not None:
             stage[1].synchronize()

@@ -91,3 +91,37 @@ def test_drafts_need_no_more_room_than_the_tokens(tmp_path, name, cache_dtype):
         assert len(got) == 83 and t["steps"] <= 82
         consistent(eng, prompt, got)
         assert not eng.runner.cache.live and eng.runner.cache.n_free_pages == eng.runner.cache.n_pages
+
+
+def test_drafts_are_gone_once_another_step_may_have_written_over_them(tmp_path, monkeypatch):
+    """A step of the request that fails in its layers, and one that is refused before anything runs."""
+    from lgml_b200.engine import ModelRunner
+    from lgml_b200.engine.runner import StepError
+
+    folder = H.make_folder(tmp_path, H.TINY_B, 1, dtype="bfloat16")
+    runner = ModelRunner.from_folder(folder, torch.bfloat16, n_pages=4, max_slots=2, max_step_tokens=64)
+    a, b = runner.open("a"), runner.open("b")
+    forward = runner.model.forward
+    tree = [(a, [1, 2], [-1, 0]), (b, [3], [-1])]
+
+    def broken(*args, **kw):
+        forward(*args, **kw)
+        raise RuntimeError("a layer failed")
+
+    for fails in (lambda: runner.step([(a, [4, 5], [0])]), lambda: runner.step_tree([(a, [6], [-1])]),
+                  lambda: runner.decode_step([a], torch.tensor([7], dtype=torch.int32, device=runner.rt.device))):
+        runner.step_tree(tree)
+        with monkeypatch.context() as m:
+            m.setattr(runner.model, "forward", broken)
+            with pytest.raises(RuntimeError, match="a layer failed"):
+                fails()
+        with pytest.raises(StepError, match="no drafted tokens"):
+            runner.keep(a, 1)
+    runner.step_tree(tree)
+    with pytest.raises(StepError):
+        runner.step([(a, [320], [0])])
+    runner.step([(b, [9], [0])])
+    runner.keep(a, 2)
+    assert (a.n_tokens, b.n_tokens) == (2, 1)
+    with pytest.raises(StepError):
+        runner.keep(b, 1)
