@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const float *
     }
     // ---- and the slices ----
     if (n_slices > 1) {
+        __syncwarp();                   // (the barrier takes whole warps)
         cluster_sync();
         if (slice == 0) {
             for (int i = tid; i < n_slices * top; i += THREADS) sh.list[i] = load_key_there(in_block(sh.best + i % top, i / top));
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const float *
                 sh.mine = make_float4(st.m, st.s, st.u, 0.f);
             }
         }
+        __syncwarp();
         cluster_sync();                 // (the others' shared memory is read until here)
         if (slice != 0) return;
     } else {

@@ -36,3 +36,11 @@ def test_no_block_leaves_ahead_of_the_wait(name):
         for m in re.finditer(r"\breturn;", body[:main]):
             branch = body[body.rindex("{", 0, m.start()):m.start()]
             assert "pdl_wait();" in branch, (kernel, branch)
+
+
+@pytest.mark.parametrize("name", ["attention_tree.cu", "attention_tree_tall.cu", "logprobs.cu"])
+def test_warps_come_together_ahead_of_a_cluster_barrier(name):
+    """``barrier.cluster`` is ``.aligned``: all threads of a warp have to arrive as one, and behind a branch that some of them took nothing else sees to that."""
+    for kernel, body in kernels(name):
+        for m in re.finditer(r"\bcluster_sync\(\);", body):
+            assert re.search(r"__sync(warp|threads)\(\);\s*$", body[:m.start()]), (kernel, body[m.start() - 80:m.start()])
