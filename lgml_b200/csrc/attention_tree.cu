@@ -516,10 +516,6 @@ int launch_dim(int ks, Args... args) {
 }
 }  // namespace
 
-LGML_API long long lgml_tree_attention_scratch_floats(int n_tokens, int H, int D, int n_splits) {
-    return n_splits <= MAX_CLUSTER ? 0 : (long long)n_tokens * H * n_splits * (D + 2);
-}
-
 // least, limit: requests that bring fewer or more tokens than this are left alone (their rows of out too).  k_exps null: pages in bfloat16.
 LGML_API int lgml_tree_attention(const void *q, int ldq, const int *positions, const int *seq_start, const int *seq_pos0, const long long *visible,
                                  const int *block_table, int n_seqs, int max_blocks, const void *k_pages, const void *v_pages, const void *k_exps,

@@ -170,7 +170,6 @@ constexpr int WIDE_THREADS = 256, WIDE_FROM = 65, WIDE_HEADS = 3;      // (heads
 template <int P> struct Vec;
 template <> struct Vec<2> { using type = unsigned; };
 template <> struct Vec<4> { using type = uint2; };
-template <> struct Vec<8> { using type = uint4; };
 template <int P, bool Q8, bool ADJACENT>
 __global__ void __launch_bounds__(WIDE_THREADS, Q8 && P == 4 ? 5 : 1) kv_store_wide_kernel(
     const __nv_bfloat16 *__restrict__ src, int lds, __nv_bfloat16 *__restrict__ q_out, int ldq, const int *__restrict__ positions, const int *__restrict__ cells,
