@@ -636,20 +636,6 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
 #pragma unroll
             for (int c = 0; c < PAGE; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(r.u[c]), __uint_as_float(r.u[c + 1]));
             const float largest = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_new = fmaf(largest, times, plus);
-            if (Q8) {
-                float s_new = largest * times;
-                if (page.z) {
-                    s_new = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < PAGE; ++c) s_new = fmaxf(s_new, __uint_as_float(r.u[c]) - add_s[it % RING][c]);
-                }
-                if (m_sum == -INFINITY) {
-                    m_sum = s_new;
-                } else if (s_new > m_sum + RESCALE_STEP) {
-                    l_run *= ex2(m_sum - s_new);
-                    m_sum = s_new;
-                }
-            }
             float corr = 1.f;
             if (m_ref == -INFINITY) {
                 m_ref = m_new;                       // nothing summed yet: nothing to correct
@@ -673,6 +659,49 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
                     tcgen05_st_16(lane_addr + O_COL + (uint32_t)c0, o);
                 }
             }
+            // The sum.  The probabilities below come with their values' powers of two; one factor takes those out again, unless they differ by column, or leave too
+            // little of them: then (rare) the weights are formed on their own, from the scores as they still are in tensor memory.
+            float out_of = 1.f;
+            bool apart = false;
+            if (Q8) {
+                auto raise = [&](float s_new) {
+                    if (m_sum == -INFINITY) {
+                        m_sum = s_new;
+                    } else if (s_new > m_sum + RESCALE_STEP) {
+                        l_run *= ex2(m_sum - s_new);
+                        m_sum = s_new;
+                    }
+                };
+                const bool little = m_new < m_ref - 60.f;
+                apart = page.z || (little && m_new > -INFINITY);
+                if (__any_sync(0xffffffffu, apart)) {
+                    const unsigned long long seen = edge ? (there ? seen_of(pg) : 0ull) : ~0ull;
+                    const float f = page.z ? power_of_two(unscale) : times;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < PAGE; c0 += 16) {
+                        uint32_t x[16];
+                        tcgen05_ld_16(s_addr + (uint32_t)c0, x);
+                        tcgen05_wait_ld();
+                        float most = -INFINITY, part = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float y = (seen >> (c0 + j)) & 1 ? __uint_as_float(x[j]) * f * (page.z ? kf_s[it % RING][c0 + j] : 1.f) : -INFINITY;
+                            x[j] = __float_as_uint(y);
+                            most = fmaxf(most, y);
+                        }
+                        if (apart) raise(most);
+                        const float ref = m_sum == -INFINITY ? 0.f : m_sum;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) part += ex2(__uint_as_float(x[j]) - ref);
+                        if (apart) l_run += part;
+                    }
+                }
+                if (!apart) {
+                    raise(largest * times);
+                    // (little of nothing seen: 0, whatever the factor)
+                    if (!little) out_of = ex2((m_ref == -INFINITY ? 0.f : m_ref) - plus - P_UP - (m_sum == -INFINITY ? 0.f : m_sum));
+                }
+            }
             const float less = (m_ref == -INFINITY ? plus : plus - m_ref) + P_UP;
             float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             // P over the scores, which this row's thread alone reads
@@ -693,20 +722,8 @@ __global__ void __launch_bounds__(Roles<TILES, Q8>::THREADS, TILES == 1 ? 2 : 1)
                 }
                 tcgen05_st_16(s_addr + (uint32_t)c0, packed);
             }
-            float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-            if (Q8) {
-                // The probabilities come with their values' powers: one factor takes those out again, unless they differ by column, or leave too little of them.
-                const float ref = m_sum == -INFINITY ? 0.f : m_sum;
-                const bool little = m_new < m_ref - 60.f;
-                if (page.z || (little && m_new > -INFINITY)) {
-                    sum = 0.f;
-#pragma unroll
-                    for (int c = 0; c < PAGE; ++c) sum += ex2(fmaf(__uint_as_float(r.u[c]), times, -ref) - (page.z ? add_s[it % RING][c] : 0.f));
-                } else if (!little) {             // (little of nothing seen: 0, whatever the factor)
-                    sum *= ex2((m_ref == -INFINITY ? 0.f : m_ref) - plus - P_UP - ref);
-                }
-            }
-            l_run += sum;
+            const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+            if (!apart) l_run += Q8 ? sum * out_of : sum;
             tcgen05_wait_st();
             tcgen05_fence_before();
             warp_arrive(&p_full[tile][it & 1]);
