@@ -28,9 +28,10 @@
 // values are looked at, and where one is not finite the block's products are formed one by one.
 //
 // What bounds it: with a token a request, memory, and for small caches the way there and back (a launch, a trip to the table, the cells, the join).  32 heads on 8
-// of 128, e4m3: 64 requests of up to 4,097 cells 84 us (403 MB, 4.8 TB/s: 0.73 of the measured copy rate; the requests' lengths differ, so the last
-// blocks run alone); eight of 2,176 cells 17 us (36 MB; 8.6 of them with cells on their way); one of 1,001 cells 6.8.  A tile of rows keeps two stages a warp in
-// flight, so that four blocks share an SM; more tiles three.  Taking the codes into mma.sync.m16n8k32 as they are, in place of converting them, measured
+// of 128, e4m3: 64 requests of up to 4,097 cells 86 us (403 MB, 4.7 TB/s: 0.72 of the measured copy rate; the requests' lengths differ, so the last
+// blocks run alone), of 4,096 cells each 96 (541 MB, 5.6 TB/s: 0.86); eight of 2,176 cells 17 us (36 MB; 8.6 of them with cells on their way); one of 1,001 cells 6.9.
+// (The sum of the weights by itself, ahead of the weights for the values, is 1 to 2 % of these, 6 % of four tokens of 64 requests.)  A tile of rows keeps two stages a
+// warp in flight, so that four blocks share an SM; more tiles three.  Taking the codes into mma.sync.m16n8k32 as they are, in place of converting them, measured
 // the same (the conversions hide behind the loads) and is not here.
 #include <cuda_fp16.h>
 #include <math.h>

@@ -21,17 +21,20 @@
 // Every column that a row may not see is a bit of a 64-bit word, tested only in pages that some row does not see whole.  There, values that are
 // not finite become zeros before the product (0 x NaN), and are added at the end to the rows that see them.
 //
-// What bounds it is the softmax and the conversion of the codes: exponentials and conversions share a pipe of 16 lanes a cycle, 1,024 + 512 cycles of it for 256
-// rows of a page, and a page of two tiles takes 2,200 (the tensor cores are at work for 512 of them).  Two tiles a block convert a page once for 256 rows.
+// What bounds it is the chain of a tile's softmax, page after page: 2,100 cycles from one page's scores to the next (150 until they are seen, 110 to load them, 300 for
+// scale and maximum, 1,300 for the exponentials of two warps a scheduler, 150 to hand P over), of which the products are 512.  No pipe is full: the one of the
+// exponentials and conversions is busy for 26 % of the time, the tensor cores for 23 %, an instruction is issued in 38 % of the cycles (of an SM that has a block;
+// 20 of 148 have none), and conversions by integer arithmetic, which leave that pipe alone, measured the same.  Two tiles a block convert a page once for 256 rows.
 // Three groups bring pages to two tiles, since sixteen warps are as many as leave a thread 128 registers.  Measured, four requests of up to 8,256 cells, 64
-// drafted tokens, 32 heads on 8 of 128, e4m3: 50 us (one tile a block, two threads a row, columns scaled one by one: 75; conversions by integer
-// arithmetic instead of the conversion instruction: 50; four groups at 96 registers: 59); 27 drafted tokens of one request over 2,203 cells, bfloat16: 15.3.
-// Of those 50: 2 until the queries are in, 36 for 25 pages, 4 to join the ranges; the rest is blocks that start after others.
+// drafted tokens, 32 heads on 8 of 128, e4m3: 50.4 us (one tile a block, two threads a row, columns scaled one by one: 75; four groups at 96 registers: 59); 27 drafted
+// tokens of one request over 2,203 cells, bfloat16: 15.3.  Of those 50: 2 until the queries are in, 36 for 25 pages, 4 to join the ranges; the rest is blocks
+// that start after others.  (A value that is not finite, in a page that not every row sees whole, takes its rows through the cells one by one: 420 us.)
 // Two tiles a block from 129 rows on, and a block an SM, against one tile and two blocks (us, each at its best cut; 2,064 cells, eight requests): 256 rows e4m3 38 / 58,
 // bfloat16 36 / 44, heads of 64 27 / 29; 132 rows e4m3 35 / 53, bfloat16 31 / 40; one request of 256 rows bfloat16 20 / 18; 512 rows, two of 8,256 cells: e4m3 61 / 89,
 // bfloat16 51 / 67.
 // That form is also the better one for a single tile where blocks have SMs to themselves (its second tile stays empty): 20 rows of one request e4m3 14.4 / 13.6 us, 108 of
-// one of 32,027 cells 82 / 61, bfloat16 46 / 43; not where two would share an SM: 36 rows of 64 requests of 1,009 cells 98 / 118.
+// one of 32,027 cells 82 / 61, bfloat16 46 / 43; not where two would share an SM: 36 rows of 64 requests of 1,009 cells 98 / 118.  (Both sides of these e4m3 pairs without
+// the sum's own maximum, which adds 0.5 us to two tiles' 50 and nothing to one tile's 97.)
 // Waits on mbarriers are bounded (status 14).
 #include "tree_common.cuh"
 

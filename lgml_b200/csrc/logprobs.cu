@@ -15,7 +15,7 @@
 // keys (the float's order, then the lower index first), so the order of arrival in the list changes nothing.
 // The slices of a row are a cluster, whose first block joins them, slice after slice, out of the others' shared memory.  All sums are float32.
 //
-// What bounds it is instructions (0.72 of the cycles issue one; maximum, exponential, two sums, the comparisons, a chunk's barriers and ranking), then memory:
+// What bounds it is instructions (0.67 of the cycles issue one; maximum, exponential, two sums, the comparisons, a chunk's ranking) and the chunks' barriers, then memory:
 // 1,021 rows of 128,256 logits with 20 alternatives take 130 us (524 MB, 4.0 TB/s, 0.61 of the measured copy rate; without alternatives 86, 0.93); 8 rows 12.5 us, a cluster of 16 blocks a row.
 // For those 1,021 rows: loads through registers and a ranking with every chunk 179; PER_SM blocks an SM: 2 224, 3 175, 4 133, 5 138, 6 190 (registers spill); two
 // stages 133; the list ranked with every entry that comes 132, from RANK_AT = 16 on 133, from 64 on 140 (what it saves is barriers where few entries come).

@@ -2933,8 +2933,8 @@ E4M3 = torch.float8_e4m3fn
 TREE_TOKENS = 64            # most new tokens of a request that ``tree_attention`` takes (bits of a mask)
 TREE_MAX_DIM = 128
 # Rows of a KV head (tokens x heads) from which ``tree_attention`` takes 128 or 256 of them a block, on tcgen05; the second number where there are more e4m3
-# pages' KV heads than SMs (us there and on mma.sync, 32 heads on 8 of 128, 2,000 cells; 16 rows: one request 14 / 13, eight 31 / 21; 20 rows: bfloat16, one 13 / 18,
-# eight 26 / 35, 64 148 / 173; e4m3 15 / 18, 31 / 31, 174 / 146; 32 rows: e4m3 15 / 20, 31 / 36, 177 / 154; 36 rows: 15 / 24, 31 / 52).
+# pages' KV heads than SMs (us there and on mma.sync, 32 heads on 8 of 128, 2,000 cells; 16 rows: one request 15 / 13, eight 29 / 30; 20 rows: bfloat16, one 13 / 18,
+# eight 24 / 36, 64 148 / 170; e4m3 15 / 20, 29 / 33, 173 / 165; 32 rows: e4m3 15 / 23, 29 / 37, 173 / 174; 36 rows: 15 / 25, 29 / 57).
 TREE_TALL_ROWS = (17, 33)
 TREE_CLUSTER = 8            # ranges of a request's pages that join without scratch memory
 LOGPROBS_TOP = 32           # most alternatives of ``token_logprobs``
@@ -3098,9 +3098,9 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exps: torch.Tensor, 
 def tree_splits(n_seqs: int, n_kv_heads: int, rows: int, longest: int, page: int = 64, tall: bool = False) -> int:
     """Into how many ranges of pages ``tree_attention`` cuts a request's cells: as many as fill the SMs with its blocks, two pages at least each; up to 8 join in
     one kernel, more cost a second one (4 us) and are taken for 128 pages and more, of eight pages each.  (32 heads on 8 of 128, e4m3, us: one request of 1,001
-    cells 15 in one range, 7 in 6 to 8, 8 in 16; of 8,001 cells 17 in 8, 14 in 16, 19 in 48; of 32,001 52 in 8, 29 in 62; eight of 2,176 29, 17 in 6 to 8, 21 in
-    16; 16 of 4,001 60, 30 in 4, 37 in 8; 64 of up to 4,097 85, 84 in 2, 120 in 8; 128 of 2,001 97, 107 in 2.  With 64 drafted tokens, four requests of up to 8,256
-    155, 84 in 2, 50 in 4, 88 in 8; 36 rows of eight requests of 2,009 50, 32 in 2, 31 in 4, 44 in 8; 108 rows of 16, bfloat16, 37, 50 in 2.)"""
+    cells 15 in one range, 7 to 8 in 6 to 8, 8 in 16; of 8,001 cells 18 in 8, 14 in 16, 20 in 48; of 32,001 52 in 8, 33 in 62; eight of 2,176 29, 16 to 17 in 6 to 8, 21 in
+    16; 16 of 4,001 55, 31 in 4, 39 in 8; 64 of up to 4,097 86, 85 in 2, 118 in 8; 128 of 2,001 98, 108 in 2.  With 64 drafted tokens, four requests of up to 8,256
+    149, 83 in 2, 50 in 4, 91 in 8; 36 rows of eight requests of 2,009 46, 29 in 2 and in 4, 42 in 8; 108 rows of 16, bfloat16, 37, 50 in 2.)"""
     height, per_sm = (256 if rows > 128 else 128, 1) if tall else (8, 4) if rows <= 8 else (16, 4) if rows <= 16 else (32, 2)
     blocks = max(n_seqs * n_kv_heads * -(-rows // height), 1)
     pages = max(1, -(-longest // page))
@@ -3133,7 +3133,8 @@ def tree_attention(q: torch.Tensor, positions: torch.Tensor, seq_start: torch.Te
     Requests that bring fewer than ``min_new_tokens`` or more than ``max_new_tokens`` are left alone, their rows of ``out`` too.  ``max_kv_len``: the longest context, new tokens
     included; it decides the ranges a request's cells are cut into (``n_splits`` otherwise), not what is read.  Positions, first rows, counts, masks and the
     block table are a step's description, which is complete before the kernels ahead are launched.  Results depend on the number of ranges and on the kernel
-    that the rows take in their rounding only; one call's are the same each time."""
+    that the rows take in their rounding only; one call's are the same each time.  Weights and their sum are float32, and a weight below 2^-126 of its row's largest is none;
+    beside a value a weight is rounded once, to bfloat16 (2^-8), or with exponents to float16 (2^-11; products below 2^-21 of the row's largest to 2^-32 of that)."""
     who = "tree_attention"
     dev = _device_of(who, k_pages, "key pages")
     n_pages, hkv, page, d = _kv_pages(who, dev, k_pages, v_pages, k_exps, v_exps)
@@ -3182,7 +3183,7 @@ def cached_attention(q, batch, cache, out, n_heads: int, scale: float, window: i
     if visible is not None and len(short) < len(batch.seq_lens):
         raise KernelError(f"cached_attention: a tree has at most {TREE_TOKENS} tokens, a request brings {batch.max_q_len}")
     # Many requests of a token or a few beside one of many: each kind by the kernel that suits its rows (a block of 256 rows takes three times as long over a single
-    # token's four as one of eight does: 64 requests of up to 4,096 cells beside one of 64 new tokens 331 us in one call, 136 in two; 20 of them 154 and 64).
+    # token's four as one of eight does: 64 requests of up to 4,096 cells beside one of 64 new tokens 319 us in one call, 142 in two; 20 of them 148 and 67).
     few = [n for n in short if n * (n_heads // k.shape[1]) < TREE_TALL_ROWS[0]]
     parts = [(1, few), (max(few) + 1, [n for n in short if n > max(few)])] if few and len(few) < len(short) and len(few) * k.shape[1] > sm_count() else [(1, short)]
     for least, lens in parts:
